@@ -379,6 +379,136 @@ rnntStatus_t rnnt_row_argmax(const void *x, int rows, int V, rnntDtype_t dtype, 
 rnntStatus_t rnnt_row_max_logp(const void *x, int rows, int V, rnntDtype_t dtype, int *out, float *logp,
                                void *stream);
 
+/*
+ * The same two under decoding rules: x'[r, v] replaces x[r, v] before the maximum is taken, in this order, in fp32:
+ *   c = how often v stands in the row's history:  if c > 0:  x' = x' > 0 ? x' / repetition_penalty : x' * repetition_penalty
+ *   x' -= frequency_penalty * c + (c > 0 ? presence_penalty : 0) (as two subtractions);  x' += bias[v];
+ *   v not allowed: x' = -inf (whatever x holds there, NaN included).
+ * The reference decodes from the raw logits (src/rnnt/model.py:152-153, src/rnnt/beam_searcher.py:91-93); blank is
+ * never in a history of emitted symbols, so the penalties leave it alone.
+ * Row r belongs to context r / (rows / contexts): the frames of an utterance's window share its history, its bias and
+ * its mask.  rows must be a multiple of contexts.
+ *   history       int32 [contexts, history_stride], the first history_lens[c] of every row count (at most
+ *                 history_stride; history_lens NULL: all of them); entries outside [0, V) are ignored; NULL: none
+ *   bias          fp32, bias_stride elements between contexts (0: one row for all); NULL: none
+ *   allowed       one bit per token, token v in bit v % 32 of word v / 32; allowed_stride words between contexts (0: one
+ *                 row for all), at least (V + 31) / 32 words per row; NULL: all allowed
+ * rnnt_row_rules writes out / logp (logp may be NULL) as rnnt_row_max_logp does: a row that its mask empties gives
+ * token 0 and a NaN score, as a row of -inf there.  rnnt_process_logits writes x' itself, rounded to the logits' type
+ * once; processed may be x (in place).
+ * history_stride <= RNNT_MAX_HISTORY (the counters hold 16 bits).
+ */
+#define RNNT_MAX_HISTORY 65535
+typedef struct {
+    int contexts;
+    const int *history;
+    const int *history_lens;
+    int history_stride;
+    const float *bias;
+    long long bias_stride;
+    const int *allowed;
+    long long allowed_stride;
+    float repetition_penalty, presence_penalty, frequency_penalty;
+} rnntRules;
+rnntStatus_t rnnt_row_rules(const void *x, int rows, int V, rnntDtype_t dtype, const rnntRules *rules, int *out,
+                            float *logp, void *stream);
+rnntStatus_t rnnt_process_logits(const void *x, int rows, int V, rnntDtype_t dtype, const rnntRules *rules,
+                                 void *processed, void *stream);
+
+/*
+ * ---- the prediction network's layers ------------------------------------------------------------------------------
+ * The reference's prediction network is embedding -> LSTM -> Linear (src/decoder/decoder.py:5-44).
+ *
+ * Token embedding (src/decoder/decoder.py:9): out[i, :] = scale * weight[tokens[i], :], rounded once; tokens are int32 or int64
+ * (tokens_64 = 1), weight rows weight_stride elements apart, out [n, dim] contiguous.  A token outside [0, vocab) gives a
+ * row of NaN.  backward: grad_weight[v, :] = scale * (sum of grad_out[i, :] over the positions i with tokens[i] = v, in
+ * position order, fp32), rounded once, for EVERY v in [0, vocab): zeros where no position holds v, and for
+ * v = padding_idx (-1: none); tokens outside [0, vocab) add nothing.  grad_out rows are grad_stride elements apart.  No
+ * atomics.  workspace: rnnt_token_embedding_workspace_size bytes, 16-byte aligned.  n < 2^31 - 2^16.
+ */
+rnntStatus_t rnnt_token_embedding_forward(const void *tokens, int tokens_64, long long n, const void *weight,
+                                          long long weight_stride, int vocab, int dim, float scale, rnntDtype_t dtype,
+                                          void *out, void *stream);
+rnntStatus_t rnnt_token_embedding_workspace_size(long long n, int vocab, int dim, size_t *size_bytes);
+rnntStatus_t rnnt_token_embedding_backward(const void *tokens, int tokens_64, long long n, const void *grad_out,
+                                           long long grad_stride, int vocab, int dim, float scale, long long padding_idx,
+                                           rnntDtype_t dtype, void *grad_weight, void *workspace, void *stream);
+
+/*
+ * Causal convolution over time, one filter per channel:
+ *   xe = [initial_state (width - 1 rows); x]      p[t, d] = bias[d] + sum_k weight[d, k] xe[t + k, d]
+ *   y[t, d] = silu ? p sigmoid(p) : p             final_state = xe[len .. len + width - 1)
+ * x [batch, length, dim] with strides x_batch / x_time (elements; channels adjacent), y [batch, length, dim] contiguous,
+ * states [batch, width - 1, dim] contiguous in x's type, weight [dim, width] and bias [dim] (NULL: none) fp32; 2 <= width <= 4.
+ * lengths int32 [batch] (NULL: all `length`; values are clamped to [0, length]): rows from lengths[b] on are not read,
+ * y there is zero.  initial_state NULL: zeros.  final_state may be NULL, or the buffer of initial_state (in place).
+ * backward: grad_x / grad_initial in x's type, grad_weight [dim, width] / grad_bias [dim] fp32; grad_final (gradient of
+ * final_state, NULL: none), grad_initial and grad_bias may be NULL.
+ * workspace: rnnt_causal_conv_workspace_size bytes, 16-byte aligned.
+ * step: one row per sequence, x [batch, dim] (x_batch apart); state_out may be the buffer of state (in place).
+ */
+typedef struct {
+    int batch, length, dim, width, silu, dtype;
+    const void *x;
+    long long x_batch, x_time;
+    const float *weight, *bias;
+    const void *initial_state;
+    const int *lengths;
+    void *y, *final_state;
+    /* backward only */
+    const void *grad_y;
+    long long grad_y_batch, grad_y_time;
+    const void *grad_final;
+    void *grad_x;
+    float *grad_weight, *grad_bias;
+    void *grad_initial;
+    void *workspace;
+    void *stream;
+} rnntConv;
+rnntStatus_t rnnt_causal_conv_forward(const rnntConv *conv);
+rnntStatus_t rnnt_causal_conv_workspace_size(int batch, int length, int dim, int width, size_t *size_bytes);
+rnntStatus_t rnnt_causal_conv_backward(const rnntConv *conv);
+rnntStatus_t rnnt_causal_conv_step(const rnntConv *conv);
+
+/*
+ * Selective scan:
+ *   delta = softplus(dt + dt_bias)     h[t, d, n] = exp(delta A[d, n]) h[t-1, d, n] + delta x[t, d] B[t, n]
+ *   y[t, d] = (sum_n C[t, n] h[t, d, n] + D[d] x[t, d]) * (z ? z sigmoid(z) : 1)
+ * x, dt, z, [batch, length, dim] and B, C [batch, length, state] of one type, each with its strides (batch, time;
+ * last dimension adjacent); A [dim, state], D, dt_bias [dim] fp32; initial_state, final_state [batch, dim, state]
+ * fp32 contiguous; y contiguous.  state is 8, 16 or 32.  D, z, dt_bias, initial_state, final_state, lengths may be NULL
+ * (lengths as above; a length of 0 gives back the initial state).
+ * forward: chunk_states (NULL in inference) receives the state before every 16th step, rnnt_selective_scan_states_size
+ * bytes, which backward reads.  backward: grad_y [batch, length, dim] (strides), grad_final NULL or contiguous;
+ * grad_x, grad_dt, grad_z (NULL iff z is NULL) and grad_B, grad_C contiguous in the inputs' type, zero from lengths[b] on;
+ * grad_A, grad_D, grad_dt_bias fp32 (the latter two may be NULL), grad_initial may be NULL.
+ * workspace: rnnt_selective_scan_workspace_size bytes (0: may be NULL), 16-byte aligned, for forward and backward alike.
+ * step: one token per sequence (length is ignored, times strides too); reads initial_state (required), writes final_state
+ * (required; may be the same buffer).
+ */
+typedef struct {
+    int batch, length, dim, state, dtype;
+    const void *x, *dt, *z, *B, *C;
+    long long x_batch, x_time, dt_batch, dt_time, z_batch, z_time, B_batch, B_time, C_batch, C_time;
+    const float *A, *D, *dt_bias, *initial_state;
+    const int *lengths;
+    void *y;
+    float *final_state, *chunk_states;
+    /* backward only */
+    const void *grad_y;
+    long long grad_y_batch, grad_y_time;
+    const float *grad_final;
+    void *grad_x, *grad_dt, *grad_z, *grad_B, *grad_C;
+    float *grad_A, *grad_D, *grad_dt_bias, *grad_initial;
+    void *workspace;
+    void *stream;
+} rnntScan;
+rnntStatus_t rnnt_selective_scan_states_size(int batch, int length, int dim, int state, size_t *size_bytes);
+rnntStatus_t rnnt_selective_scan_workspace_size(int batch, int length, int dim, int state, int backward, size_t *size_bytes);
+rnntStatus_t rnnt_selective_scan_forward(const rnntScan *scan);
+rnntStatus_t rnnt_selective_scan_backward(const rnntScan *scan);
+rnntStatus_t rnnt_selective_scan_step(const rnntScan *scan);
+
 /* hipEvent helpers so a ctypes caller (bench.py) can time stages without a HIP binding. */
 rnntStatus_t rnnt_event_create(void **event);
 rnntStatus_t rnnt_event_destroy(void *event);

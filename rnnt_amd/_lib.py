@@ -58,6 +58,20 @@ EXPORTED_SYMBOLS = (
     "rnnt_joint_hidden_backward_compact",
     "rnnt_row_argmax",
     "rnnt_row_max_logp",
+    "rnnt_row_rules",
+    "rnnt_process_logits",
+    "rnnt_token_embedding_forward",
+    "rnnt_token_embedding_workspace_size",
+    "rnnt_token_embedding_backward",
+    "rnnt_causal_conv_forward",
+    "rnnt_causal_conv_workspace_size",
+    "rnnt_causal_conv_backward",
+    "rnnt_causal_conv_step",
+    "rnnt_selective_scan_states_size",
+    "rnnt_selective_scan_workspace_size",
+    "rnnt_selective_scan_forward",
+    "rnnt_selective_scan_backward",
+    "rnnt_selective_scan_step",
     "rnnt_event_create",
     "rnnt_event_destroy",
     "rnnt_event_record",
@@ -76,6 +90,43 @@ class RnntOptions(ctypes.Structure):
         ("dtype", ctypes.c_int),
         ("stage_events", ctypes.POINTER(ctypes.c_void_p)),
     ]
+
+
+class RnntRules(ctypes.Structure):
+    """Mirror of ``rnntRules`` (include/rnnt_mi355.h)."""
+
+    _fields_ = [("contexts", ctypes.c_int), ("history", ctypes.c_void_p), ("history_lens", ctypes.c_void_p),
+                ("history_stride", ctypes.c_int), ("bias", ctypes.c_void_p), ("bias_stride", ctypes.c_longlong),
+                ("allowed", ctypes.c_void_p), ("allowed_stride", ctypes.c_longlong), ("repetition_penalty", ctypes.c_float),
+                ("presence_penalty", ctypes.c_float), ("frequency_penalty", ctypes.c_float)]
+
+
+def _struct_fields(text):
+    """``"i:a b p:c"`` -> ctypes fields, i int, l long long, p pointer."""
+    kinds = {"i": ctypes.c_int, "l": ctypes.c_longlong, "p": ctypes.c_void_p}
+    fields, kind = [], None
+    for word in text.split():
+        if word[1:2] == ":":
+            kind, word = kinds[word[0]], word[2:]
+        fields.append((word, kind))
+    return fields
+
+
+class RnntConv(ctypes.Structure):
+    """Mirror of ``rnntConv`` (include/rnnt_mi355.h)."""
+
+    _fields_ = _struct_fields("i:batch length dim width silu dtype p:x l:x_batch x_time p:weight bias initial_state lengths y "
+                              "final_state grad_y l:grad_y_batch grad_y_time p:grad_final grad_x grad_weight grad_bias "
+                              "grad_initial workspace stream")
+
+
+class RnntScan(ctypes.Structure):
+    """Mirror of ``rnntScan`` (include/rnnt_mi355.h)."""
+
+    _fields_ = _struct_fields("i:batch length dim state dtype p:x dt z B C l:x_batch x_time dt_batch dt_time z_batch z_time "
+                              "B_batch B_time C_batch C_time p:A D dt_bias initial_state lengths y final_state chunk_states "
+                              "grad_y l:grad_y_batch grad_y_time p:grad_final grad_x grad_dt grad_z grad_B grad_C grad_A "
+                              "grad_D grad_dt_bias grad_initial workspace stream")
 
 
 class RnntLibraryError(RuntimeError):
@@ -197,6 +248,20 @@ def load() -> ctypes.CDLL:
         lib.rnnt_row_argmax.restype = ctypes.c_int
         lib.rnnt_row_max_logp.argtypes = [vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, vp, vp, ctypes.c_void_p]
         lib.rnnt_row_max_logp.restype = ctypes.c_int
+        lib.rnnt_row_rules.argtypes = [vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.POINTER(RnntRules), vp, vp, vp]
+        lib.rnnt_process_logits.argtypes = [vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.POINTER(RnntRules), vp, vp]
+        lib.rnnt_token_embedding_forward.argtypes = [vp, ctypes.c_int, ctypes.c_longlong, vp, ctypes.c_longlong, ctypes.c_int,
+                                                     ctypes.c_int, ctypes.c_float, ctypes.c_int, vp, vp]
+        lib.rnnt_token_embedding_workspace_size.argtypes = [ctypes.c_longlong, ctypes.c_int, ctypes.c_int,
+                                                            ctypes.POINTER(ctypes.c_size_t)]
+        lib.rnnt_token_embedding_backward.argtypes = [vp, ctypes.c_int, ctypes.c_longlong, vp, ctypes.c_longlong, ctypes.c_int,
+                                                      ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_int, vp, vp, vp]
+        lib.rnnt_causal_conv_workspace_size.argtypes = [ctypes.c_int] * 4 + [ctypes.POINTER(ctypes.c_size_t)]
+        lib.rnnt_selective_scan_states_size.argtypes = [ctypes.c_int] * 4 + [ctypes.POINTER(ctypes.c_size_t)]
+        lib.rnnt_selective_scan_workspace_size.argtypes = [ctypes.c_int] * 5 + [ctypes.POINTER(ctypes.c_size_t)]
+        for name in ("forward", "backward", "step"):
+            getattr(lib, "rnnt_causal_conv_" + name).argtypes = [ctypes.POINTER(RnntConv)]
+            getattr(lib, "rnnt_selective_scan_" + name).argtypes = [ctypes.POINTER(RnntScan)]
         lib.rnnt_event_create.argtypes = [ctypes.POINTER(ctypes.c_void_p)]
         lib.rnnt_event_create.restype = ctypes.c_int
         lib.rnnt_event_destroy.argtypes = [ctypes.c_void_p]

@@ -1,0 +1,461 @@
+// embedding_mi355.hip — token embedding of a prediction network on MI355X (gfx950): the lookup with its scale, and its
+// gradient by sorted tokens.
+//
+// The reference's prediction network begins with nn.Embedding (src/decoder/decoder.py:9).  Forward copies one row per
+// token.  Backward sums the gradient rows of each token.  Adding them with atomics would let their order, and with it the
+// last bits, vary from run to run, and would serialise on the frequent tokens (a label sequence is full of them);
+// instead the positions are sorted by token first (stable: position order), the sorted list is cut into equal pieces
+// whatever the tokens' frequencies, each piece sums its runs of equal tokens in fp32 registers, and the runs that
+// cross pieces are joined in order.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/rnnt_mi355.h"
+#include "elem_types.h"
+
+namespace {
+
+using namespace rnnt_mi355_detail;
+
+constexpr int kBlock = 256;
+constexpr int kPiece = 32;        // sorted positions per piece
+constexpr int kRankMax = 4096;    // up to this many positions are sorted by counting smaller ones
+constexpr int kSortItems = 4096;  // positions per workgroup and pass of the radix sort
+constexpr int kDigits = 256;
+
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+__device__ __forceinline__ long long token_at(const void *tokens, int tokens_64, long long i) {
+    return tokens_64 ? static_cast<const long long *>(tokens)[i] : (long long)static_cast<const int *>(tokens)[i];
+}
+
+// sort key: the token, or `vocab` (last) for a position that adds to no row
+__device__ __forceinline__ int key_at(const void *tokens, int tokens_64, long long i, int vocab, long long padding) {
+    const long long t = token_at(tokens, tokens_64, i);
+    return t >= 0 && t < vocab && t != padding ? (int)t : vocab;
+}
+
+// a lane's piece of a row: VEC elements
+template <typename DT, int VEC>
+__device__ __forceinline__ void load_piece(const typename DT::elem *p, float (&f)[VEC]) {
+    if constexpr (VEC == 1)
+        f[0] = DT::to_float(*p);
+    else
+        DT::unpack(*reinterpret_cast<const u32x4 *>(p), f);
+}
+template <typename DT, int VEC>
+__device__ __forceinline__ void store_piece(typename DT::elem *p, const float (&f)[VEC]) {
+    if constexpr (VEC == 1)
+        *p = DT::from_float(f[0]);
+    else
+        *reinterpret_cast<u32x4 *>(p) = DT::pack(f);
+}
+
+// Rows are shared out to groups of 2^shift lanes; a group walks its row in pieces of VEC elements per lane.
+template <typename DT, int VEC>
+__global__ __launch_bounds__(kBlock) void embed_forward_kernel(const void *__restrict__ tokens, int tokens_64, long long n,
+                                                               const typename DT::elem *__restrict__ weight,
+                                                               long long weight_stride, int vocab, int dim, float scale,
+                                                               typename DT::elem *__restrict__ out, int shift) {
+    const int sub = threadIdx.x & ((1 << shift) - 1);
+    const long long i = ((long long)blockIdx.x * kBlock + threadIdx.x) >> shift;
+    if (i >= n) return;
+    const long long t = token_at(tokens, tokens_64, i);
+    const bool ok = t >= 0 && t < vocab;
+    const typename DT::elem *row = weight + (ok ? t : 0) * weight_stride;
+    for (int c = sub * VEC; c < dim; c += VEC << shift) {
+        float f[VEC];
+        load_piece<DT, VEC>(row + c, f);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f[j] = ok ? f[j] * scale : __builtin_nanf("");
+        store_piece<DT, VEC>(out + (size_t)i * dim + c, f);
+    }
+}
+
+// ---- sorting ---------------------------------------------------------------------------------------------------------
+// Few positions: a position's place is the number of positions before it in the order, counted against all others.
+// n^2 comparisons over n / 256 workgroups in one launch, nothing to wait for.
+__global__ __launch_bounds__(kBlock) void embed_rank_kernel(const void *__restrict__ tokens, int tokens_64, int n, int vocab,
+                                                            long long padding, int *__restrict__ sorted, int *__restrict__ order) {
+    __shared__ int s_key[kRankMax];
+    for (int j = threadIdx.x; j < n; j += kBlock) s_key[j] = key_at(tokens, tokens_64, j, vocab, padding);
+    __syncthreads();
+    const int i = blockIdx.x * kBlock + threadIdx.x;
+    if (i >= n) return;
+    const int key = s_key[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += s_key[j] < key || (s_key[j] == key && j < i);
+    sorted[rank] = key;
+    order[rank] = i;
+}
+
+// Many positions: radix sort from the lowest digit, 8 bits per pass, two launches per pass.  A workgroup's wave w owns
+// its w-th quarter; lanes with the same digit find each other with 8 ballots, so that ranks follow the position.
+template <bool FIRST>
+__device__ __forceinline__ int sort_key(const void *src, int tokens_64, long long i, int vocab, long long padding) {
+    return FIRST ? key_at(src, tokens_64, i, vocab, padding) : static_cast<const int *>(src)[i];
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(kBlock) void embed_digit_kernel(const void *__restrict__ src, int tokens_64, int n, int vocab,
+                                                             long long padding, int bit, int *__restrict__ counts) {
+    __shared__ int s_count[kDigits];
+    s_count[threadIdx.x] = 0;
+    __syncthreads();
+    const long long base = (long long)blockIdx.x * kSortItems;
+    for (int k = threadIdx.x; k < kSortItems; k += kBlock)
+        if (base + k < n) atomicAdd(&s_count[(sort_key<FIRST>(src, tokens_64, base + k, vocab, padding) >> bit) & (kDigits - 1)], 1);
+    __syncthreads();
+    counts[(size_t)blockIdx.x * kDigits + threadIdx.x] = s_count[threadIdx.x];
+}
+
+__device__ __forceinline__ unsigned long long same_digit(int digit, bool live) {
+    unsigned long long peers = __ballot(live);
+#pragma unroll
+    for (int bit = 0; bit < 8; ++bit) {
+        const unsigned long long set = __ballot((digit >> bit) & 1);
+        peers &= (digit >> bit) & 1 ? set : ~set;
+    }
+    return peers;
+}
+
+template <bool FIRST>
+__global__ __launch_bounds__(kBlock) void embed_place_kernel(const void *__restrict__ src, int tokens_64, int n, int vocab,
+                                                             long long padding, int bit, const int *__restrict__ counts,
+                                                             const int *__restrict__ order_in, int *__restrict__ sorted,
+                                                             int *__restrict__ order) {
+    constexpr int kWaves = kBlock / kWave, kRounds = kSortItems / kBlock;
+    __shared__ int s_base[kWaves][kDigits];
+    __shared__ int s_total[kDigits];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const long long base = (long long)blockIdx.x * kSortItems + wave * (kSortItems / kWaves);
+    int before = 0, total = 0;  // of digit threadIdx.x: in the workgroups before this one, in all
+    for (int w = 0; w < (int)gridDim.x; ++w) {
+        const int c = counts[(size_t)w * kDigits + threadIdx.x];
+        before += w < (int)blockIdx.x ? c : 0;
+        total += c;
+    }
+    s_total[threadIdx.x] = total;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) s_base[w][threadIdx.x] = 0;
+    __syncthreads();
+    for (int step = 1; step < kDigits; step <<= 1) {  // inclusive sums over the digits
+        const int v = (int)threadIdx.x >= step ? s_total[threadIdx.x - step] : 0;
+        __syncthreads();
+        s_total[threadIdx.x] += v;
+        __syncthreads();
+    }
+    int key[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        const long long i = base + r * kWave + lane;
+        key[r] = i < n ? sort_key<FIRST>(src, tokens_64, i, vocab, padding) : -1;
+        if (i < n) atomicAdd(&s_base[wave][(key[r] >> bit) & (kDigits - 1)], 1);
+    }
+    __syncthreads();
+    {
+        int at = s_total[threadIdx.x] - total + before;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const int c = s_base[w][threadIdx.x];
+            s_base[w][threadIdx.x] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+        const long long i = base + r * kWave + lane;
+        const bool live = i < n;
+        const int digit = (key[r] >> bit) & (kDigits - 1);
+        const unsigned long long peers = same_digit(digit, live);
+        const int ahead = __popcll(peers & ((1ull << lane) - 1));
+        int at = 0;
+        if (live) at = s_base[wave][digit] + ahead;
+        // (a wave's LDS accesses stay in order: all lanes have read before the first of each digit moves its base on)
+        __builtin_amdgcn_wave_barrier();
+        if (live && ahead == 0) s_base[wave][digit] += __popcll(peers);
+        __builtin_amdgcn_wave_barrier();
+        if (live) {
+            sorted[at] = key[r];
+            order[at] = FIRST ? (int)i : order_in[i];
+        }
+    }
+}
+
+// ---- sums ------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ int lower_bound(const int *sorted, int n, int key) {
+    int lo = 0, hi = n;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sorted[mid] < key)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+// Groups [0, pieces): a piece of sorted positions each.  A run of equal tokens inside the piece is written out; the part
+// of a run that began in an earlier piece goes to partial[piece][0], the part of one that begins here and goes on to
+// partial[piece][1].  Groups [pieces, pieces + vocab): the rows of tokens that no position holds are set to zero.
+template <typename DT, int VEC>
+__global__ __launch_bounds__(kBlock) void embed_sum_kernel(const int *__restrict__ sorted, const int *__restrict__ order, int n,
+                                                           const typename DT::elem *__restrict__ grad, long long grad_stride,
+                                                           int vocab, int dim, float scale,
+                                                           typename DT::elem *__restrict__ grad_weight,
+                                                           float *__restrict__ partial, int pieces, int shift) {
+    const int sub = threadIdx.x & ((1 << shift) - 1);
+    const long long group = ((long long)blockIdx.x * kBlock + threadIdx.x) >> shift;
+    const int width = VEC << shift;
+    if (group >= pieces) {
+        const long long v = group - pieces;
+        if (v >= vocab) return;
+        const int at = lower_bound(sorted, n, (int)v);
+        if (at < n && sorted[at] == (int)v) return;
+        const float zero[VEC] = {};
+        for (int c = sub * VEC; c < dim; c += width) store_piece<DT, VEC>(grad_weight + (size_t)v * dim + c, zero);
+        return;
+    }
+    const int begin = (int)group * kPiece, end = begin + kPiece < n ? begin + kPiece : n;
+    const int prev = begin > 0 ? sorted[begin - 1] : -1, next = end < n ? sorted[end] : -1;
+    for (int c = sub * VEC; c < dim; c += width) {
+        float acc[VEC] = {};
+        int cur = sorted[begin];
+        bool from_before = cur == prev;
+        auto close = [&](bool goes_on) {
+            if (cur == vocab) return;
+            if (from_before || goes_on) {
+                float *p = partial + ((size_t)group * 2 + (from_before ? 0 : 1)) * dim + c;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) p[j] = acc[j];
+            } else {
+                float f[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) f[j] = acc[j] * scale;
+                store_piece<DT, VEC>(grad_weight + (size_t)cur * dim + c, f);
+            }
+        };
+        for (int k = begin; k < end; ++k) {
+            const int tok = sorted[k];
+            if (tok != cur) {
+                close(false);
+                cur = tok;
+                from_before = false;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+            }
+            if (tok == vocab) break;
+            float f[VEC];
+            load_piece<DT, VEC>(grad + (size_t)order[k] * grad_stride + c, f);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) acc[j] += f[j];
+        }
+        close(cur == next);
+    }
+}
+
+// The runs that cross pieces: the workgroup of the piece a run begins in adds the run's parts, each wave a range of
+// the pieces in order, then the waves' sums in order.
+template <typename DT, int VEC>
+__global__ __launch_bounds__(kBlock) void embed_join_kernel(const int *__restrict__ sorted, int n, int vocab, int dim, float scale,
+                                                            typename DT::elem *__restrict__ grad_weight,
+                                                            const float *__restrict__ partial, int pieces) {
+    constexpr int kWaves = kBlock / kWave;
+    __shared__ float s_acc[kWaves][kWave * VEC];
+    const int piece = blockIdx.x;
+    const int begin = piece * kPiece, end = begin + kPiece;
+    if (end >= n) return;
+    const int tok = sorted[end - 1];
+    if (tok == vocab || sorted[end] != tok) return;
+    if (sorted[begin] == tok && begin > 0 && sorted[begin - 1] == tok) return;  // began earlier
+    const int stop = lower_bound(sorted, n, tok + 1);  // end of the run
+    const int last = (stop - 1) / kPiece;              // pieces piece + 1 .. last hold parts of it
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int parts = last - piece, per = (parts + kWaves - 1) / kWaves;
+    const int p0 = piece + 1 + wave * per, p1 = p0 + per < last + 1 ? p0 + per : last + 1;
+    for (int c0 = 0; c0 < dim; c0 += kWave * VEC) {
+        const int c = c0 + lane * VEC;
+        float acc[VEC] = {};
+        if (c < dim) {
+            if (wave == 0) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[j] = partial[((size_t)piece * 2 + 1) * dim + c + j];
+            }
+            for (int p = p0; p < p1; ++p)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[j] += partial[(size_t)p * 2 * dim + c + j];
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s_acc[wave][lane * VEC + j] = acc[j];
+        __syncthreads();
+        if (wave == 0 && c < dim) {
+            float f[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                float s = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w) s += s_acc[w][lane * VEC + j];
+                f[j] = s * scale;
+            }
+            store_piece<DT, VEC>(grad_weight + (size_t)tok * dim + c, f);
+        }
+        __syncthreads();
+    }
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------------
+struct EmbedSpace {
+    size_t sorted[2], order[2], counts, partial, total;
+};
+inline int pieces_of(long long n) { return (int)((n + kPiece - 1) / kPiece); }
+inline int sort_blocks(long long n) { return (int)((n + kSortItems - 1) / kSortItems); }
+inline EmbedSpace embed_space(long long n, int dim) {
+    EmbedSpace s = {};
+    size_t at = 0;
+    auto take = [&at](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 15) & ~(size_t)15;
+        return here;
+    };
+    const int copies = n > kRankMax ? 2 : 1;
+    for (int i = 0; i < copies; ++i) {
+        s.sorted[i] = take((size_t)n * 4);
+        s.order[i] = take((size_t)n * 4);
+    }
+    if (n > kRankMax) s.counts = take((size_t)sort_blocks(n) * kDigits * 4);
+    s.partial = take((size_t)pieces_of(n) * 2 * dim * 4);
+    s.total = at;
+    return s;
+}
+
+inline bool embed_shape_ok(long long n, int vocab, int dim) {
+    return n >= 1 && n < (1ll << 31) - (1 << 16) && vocab >= 1 && vocab < 0x7fffffff && dim >= 1 && dim <= (1 << 24);
+}
+
+// lanes that share a row: a power of two that covers the row's pieces, at most a wave
+inline int row_shift(int dim, int vec) {
+    int shift = 0;
+    while ((vec << shift) < dim && shift < 6) ++shift;
+    return shift;
+}
+
+template <typename DT>
+rnntStatus_t embed_forward(const void *tokens, int tokens_64, long long n, const void *weight, long long weight_stride, int vocab,
+                           int dim, float scale, void *out, hipStream_t st) {
+    typedef typename DT::elem E;
+    const bool vec = dim % DT::EPC == 0 && weight_stride % DT::EPC == 0 && aligned16(weight) && aligned16(out);
+    const int shift = row_shift(dim, vec ? DT::EPC : 1);
+    const long long blocks = ((n << shift) + kBlock - 1) / kBlock;
+    if (blocks > 0x7fffffffll) return RNNT_STATUS_INVALID_VALUE;
+    if (vec)
+        hipLaunchKernelGGL((embed_forward_kernel<DT, DT::EPC>), dim3((unsigned)blocks), dim3(kBlock), 0, st, tokens, tokens_64, n,
+                           static_cast<const E *>(weight), weight_stride, vocab, dim, scale, static_cast<E *>(out), shift);
+    else
+        hipLaunchKernelGGL((embed_forward_kernel<DT, 1>), dim3((unsigned)blocks), dim3(kBlock), 0, st, tokens, tokens_64, n,
+                           static_cast<const E *>(weight), weight_stride, vocab, dim, scale, static_cast<E *>(out), shift);
+    return hipGetLastError() == hipSuccess ? RNNT_STATUS_SUCCESS : RNNT_STATUS_EXECUTION_FAILED;
+}
+
+template <typename DT>
+rnntStatus_t embed_backward(const void *tokens, int tokens_64, long long n, const void *grad, long long grad_stride, int vocab,
+                            int dim, float scale, long long padding, void *grad_weight, void *workspace, hipStream_t st) {
+    typedef typename DT::elem E;
+    const EmbedSpace sp = embed_space(n, dim);
+    char *ws = static_cast<char *>(workspace);
+    int *sorted[2], *order[2];
+    for (int i = 0; i < 2; ++i) {
+        sorted[i] = reinterpret_cast<int *>(ws + sp.sorted[i]);
+        order[i] = reinterpret_cast<int *>(ws + sp.order[i]);
+    }
+    float *partial = reinterpret_cast<float *>(ws + sp.partial);
+    int at = 0;
+    if (n <= kRankMax) {
+        hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((n + kBlock - 1) / kBlock)), dim3(kBlock), 0, st, tokens, tokens_64,
+                           (int)n, vocab, padding, sorted[0], order[0]);
+    } else {
+        int *counts = reinterpret_cast<int *>(ws + sp.counts);
+        const dim3 grid((unsigned)sort_blocks(n));
+        hipLaunchKernelGGL((embed_digit_kernel<true>), grid, dim3(kBlock), 0, st, tokens, tokens_64, (int)n, vocab, padding, 0, counts);
+        hipLaunchKernelGGL((embed_place_kernel<true>), grid, dim3(kBlock), 0, st, tokens, tokens_64, (int)n, vocab, padding, 0,
+                           static_cast<const int *>(counts), static_cast<const int *>(nullptr), sorted[0], order[0]);
+        for (int bit = 8; bit < 31 && (vocab >> bit) != 0; bit += 8) {
+            hipLaunchKernelGGL((embed_digit_kernel<false>), grid, dim3(kBlock), 0, st, static_cast<const void *>(sorted[at]), 0, (int)n,
+                               vocab, padding, bit, counts);
+            hipLaunchKernelGGL((embed_place_kernel<false>), grid, dim3(kBlock), 0, st, static_cast<const void *>(sorted[at]), 0, (int)n,
+                               vocab, padding, bit, static_cast<const int *>(counts), static_cast<const int *>(order[at]),
+                               sorted[1 - at], order[1 - at]);
+            at = 1 - at;
+        }
+    }
+    const bool vec = dim % DT::EPC == 0 && grad_stride % DT::EPC == 0 && aligned16(grad) && aligned16(grad_weight);
+    const int shift = row_shift(dim, vec ? DT::EPC : 1);
+    const int pieces = pieces_of(n);
+    const long long blocks = ((((long long)pieces + vocab) << shift) + kBlock - 1) / kBlock;
+    if (blocks > 0x7fffffffll) return RNNT_STATUS_INVALID_VALUE;
+#define EMBED_SUM(VEC)                                                                                                       \
+    do {                                                                                                                     \
+        hipLaunchKernelGGL((embed_sum_kernel<DT, VEC>), dim3((unsigned)blocks), dim3(kBlock), 0, st,                         \
+                           static_cast<const int *>(sorted[at]), static_cast<const int *>(order[at]), (int)n,                \
+                           static_cast<const E *>(grad), grad_stride, vocab, dim, scale, static_cast<E *>(grad_weight),      \
+                           partial, pieces, shift);                                                                          \
+        if (pieces > 1)                                                                                                      \
+            hipLaunchKernelGGL((embed_join_kernel<DT, VEC>), dim3((unsigned)pieces), dim3(kBlock), 0, st,                    \
+                               static_cast<const int *>(sorted[at]), (int)n, vocab, dim, scale, static_cast<E *>(grad_weight), \
+                               static_cast<const float *>(partial), pieces);                                                 \
+    } while (0)
+    if (vec)
+        EMBED_SUM(DT::EPC);
+    else
+        EMBED_SUM(1);
+#undef EMBED_SUM
+    return hipGetLastError() == hipSuccess ? RNNT_STATUS_SUCCESS : RNNT_STATUS_EXECUTION_FAILED;
+}
+
+}  // namespace
+
+extern "C" {
+
+rnntStatus_t rnnt_token_embedding_forward(const void *tokens, int tokens_64, long long n, const void *weight,
+                                          long long weight_stride, int vocab, int dim, float scale, rnntDtype_t dtype, void *out,
+                                          void *stream) {
+    if (tokens == nullptr || weight == nullptr || out == nullptr || !embed_shape_ok(n, vocab, dim) || weight_stride < dim)
+        return RNNT_STATUS_INVALID_VALUE;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    switch (dtype) {
+        case RNNT_DTYPE_F32: return embed_forward<F32>(tokens, tokens_64, n, weight, weight_stride, vocab, dim, scale, out, st);
+        case RNNT_DTYPE_BF16: return embed_forward<BF16>(tokens, tokens_64, n, weight, weight_stride, vocab, dim, scale, out, st);
+        case RNNT_DTYPE_F16: return embed_forward<F16>(tokens, tokens_64, n, weight, weight_stride, vocab, dim, scale, out, st);
+        default: return RNNT_STATUS_INVALID_VALUE;
+    }
+}
+
+rnntStatus_t rnnt_token_embedding_workspace_size(long long n, int vocab, int dim, size_t *size_bytes) {
+    if (size_bytes == nullptr || !embed_shape_ok(n, vocab, dim)) return RNNT_STATUS_INVALID_VALUE;
+    *size_bytes = embed_space(n, dim).total;
+    return RNNT_STATUS_SUCCESS;
+}
+
+rnntStatus_t rnnt_token_embedding_backward(const void *tokens, int tokens_64, long long n, const void *grad_out,
+                                           long long grad_stride, int vocab, int dim, float scale, long long padding_idx,
+                                           rnntDtype_t dtype, void *grad_weight, void *workspace, void *stream) {
+    if (tokens == nullptr || grad_out == nullptr || grad_weight == nullptr || workspace == nullptr || !aligned16(workspace) ||
+        !embed_shape_ok(n, vocab, dim) || grad_stride < 0)
+        return RNNT_STATUS_INVALID_VALUE;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    switch (dtype) {
+        case RNNT_DTYPE_F32:
+            return embed_backward<F32>(tokens, tokens_64, n, grad_out, grad_stride, vocab, dim, scale, padding_idx, grad_weight,
+                                       workspace, st);
+        case RNNT_DTYPE_BF16:
+            return embed_backward<BF16>(tokens, tokens_64, n, grad_out, grad_stride, vocab, dim, scale, padding_idx, grad_weight,
+                                        workspace, st);
+        case RNNT_DTYPE_F16:
+            return embed_backward<F16>(tokens, tokens_64, n, grad_out, grad_stride, vocab, dim, scale, padding_idx, grad_weight,
+                                       workspace, st);
+        default: return RNNT_STATUS_INVALID_VALUE;
+    }
+}
+
+}  // extern "C"

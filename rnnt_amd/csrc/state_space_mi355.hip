@@ -1,0 +1,1076 @@
+// state_space_mi355.hip — the recurrent layer of a state-space prediction network on MI355X (gfx950): the short causal
+// convolution and the selective scan, each for whole sequences (forward and backward) and for single tokens.
+//
+// The reference's prediction network is embedding -> LSTM -> Linear (src/decoder/decoder.py:5-44) and its decoding loops
+// carry that layer's state from emission to emission (src/rnnt/model.py:145-165).  These kernels compute a layer of
+// the same place and interface:
+//     convolution   p_t = bias + sum_k w_k x_{t-W+1+k},  y_t = p_t sigmoid(p_t)
+//     scan          delta_t = softplus(dt_t + dt_bias),  h_t[n] = exp(delta_t A[n]) h_{t-1}[n] + delta_t x_t B_t[n],
+//                   y_t = (sum_n C_t[n] h_t[n] + D x_t) z_t sigmoid(z_t)
+// for every channel d of every sequence b; B_t and C_t are shared by all channels of a sequence.
+// Everything between loads and stores is fp32.  No atomics: two runs give the same bits.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "../../include/rnnt_mi355.h"
+#include "elem_types.h"
+
+namespace {
+
+using namespace rnnt_mi355_detail;
+
+constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.925963033500e-08f, kLn2 = 0.6931471805599453f;
+
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+__device__ __forceinline__ float fma_(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float rcp_(float v) { return __builtin_amdgcn_rcpf(v); }
+__device__ __forceinline__ float sigmoid_(float v) { return rcp_(1.f + exp2_(-kLog2e * v)); }
+
+// softplus(v) = max(v, 0) + log1p(e), e = exp(-|v|) in (0, 1], and its derivative sigmoid(v) in `sig`.
+// log1p(e) = e P(e), P the degree-9 Chebyshev interpolant of log1p(e) / e on [0, 1] (fit 1.2e-8 relative): rounding
+// 1 + e first would cost 6e-8 / delta, and steps of delta = 1e-3 are ordinary.  v log2(e) is formed in two parts, since
+// an exponent of 10 would pass its rounding on to delta tenfold.
+__device__ __forceinline__ float softplus_(float v, float &sig) {
+    const float w = -fabsf(v), hi = w * kLog2e;
+    float lo = fma_(w, kLog2e, -hi);
+    lo = w > -128.f ? fma_(w, kLog2eLow, lo) * kLn2 : 0.f;
+    float e = exp2_(hi);
+    e = fma_(e, lo, e);
+    float p = -3.176057013e-03f;
+    p = fma_(p, e, 1.954252832e-02f);
+    p = fma_(p, e, -5.637361482e-02f);
+    p = fma_(p, e, 1.054362357e-01f);
+    p = fma_(p, e, -1.526966691e-01f);
+    p = fma_(p, e, 1.966327429e-01f);
+    p = fma_(p, e, -2.495161593e-01f);
+    p = fma_(p, e, 3.332971036e-01f);
+    p = fma_(p, e, -4.999989271e-01f);
+    p = fma_(p, e, 1.0f);
+    const float r = rcp_(1.f + e);
+    sig = v > 0.f ? r : e * r;
+    return fma_(e, p, fmaxf(v, 0.f));  // (NaN comes through e)
+}
+
+// ---------------------------------------------------------------------------------------------
+// B_t and C_t: N adjacent values at an address that is the same for the whole wave.  They are read through the scalar
+// cache into scalar registers, so that the recurrence's multiply-adds take them as scalar operands: no vector load, no
+// LDS, no register per lane.  Scalar loads are whole 4-byte words: a row of 16-bit values that starts in the middle of
+// a word is read from that word on and moved down by 16 bits.
+// ---------------------------------------------------------------------------------------------
+typedef const __attribute__((address_space(4))) unsigned *scalar_words;
+
+template <typename DT, int N>
+struct ScalarRow {
+    static constexpr bool kHalf = sizeof(typename DT::elem) == 2;
+    static constexpr int kWords = kHalf ? N / 2 : N;
+    unsigned w[kWords];
+    __device__ __forceinline__ void load(const typename DT::elem *p) {
+        const unsigned long long at = reinterpret_cast<unsigned long long>(p);
+        scalar_words q = (scalar_words)(at & ~3ull);
+        if (!kHalf || (at & 2) == 0) {
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) w[i] = q[i];
+        } else {
+            unsigned prev = q[0];
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                const unsigned next = q[i + 1];
+                w[i] = (unsigned)(((unsigned long long)next << 32 | prev) >> 16);
+                prev = next;
+            }
+        }
+    }
+    __device__ __forceinline__ float operator[](int n) const {
+        if constexpr (!kHalf) {
+            return __uint_as_float(w[n]);
+        } else {
+            const unsigned v = w[n / 2];
+            if constexpr (sizeof(DT) && __is_same(DT, BF16)) {
+                return __uint_as_float(n & 1 ? v & 0xffff0000u : v << 16);
+            } else {
+                return (float)__builtin_bit_cast(_Float16, (unsigned short)(n & 1 ? v >> 16 : v & 0xffffu));
+            }
+        }
+    }
+};
+
+// ---------------------------------------------------------------------------------------------
+// selective scan
+// ---------------------------------------------------------------------------------------------
+constexpr int kChunk = 16;  // steps between saved states; steps a backward wave holds in registers
+constexpr int kAhead = 4;   // steps whose inputs a forward wave loads ahead
+
+// A channel's constants and where a wave works.  Segments cut the time axis so that few sequences fill the chip:
+// pass 1 walks every segment from a zero state (`local`), pass 2 joins the segments' ends in order, pass 3 walks them
+// again from the right states.  A single segment needs pass 3 alone.
+struct ScanGeom {
+    int groups;    // of 64 channels
+    int segments;  // per sequence
+    int seg_len;   // steps per segment, a multiple of kChunk
+    float *seg_state;  // [batch][segments][state / 4][dim][4]: a segment's end from zero, then the state it starts from
+    float *seg_delta;  // [batch][segments][dim]: sum of delta over the segment
+};
+
+__device__ __forceinline__ int clamp_len(const int *lengths, int b, int length) {
+    if (lengths == nullptr) return length;
+    const int n = lengths[b];
+    return n < 0 ? 0 : (n > length ? length : n);
+}
+
+template <int N>
+__device__ __forceinline__ void load_rates(const float *A, int d, float (&A2)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) A2[n] = A[(size_t)d * N + n] * kLog2e;
+}
+
+// state tiles between kernels: [N / 4][dim][4] per (sequence, time)
+template <int N>
+__device__ __forceinline__ void load_tile(const float *tile, int dim, int d, float (&h)[N]) {
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+        const f32x2 *p = reinterpret_cast<const f32x2 *>(tile + ((size_t)q * dim + d) * 4);
+        const f32x2 lo = p[0], hi = p[1];
+        h[4 * q] = lo.x;
+        h[4 * q + 1] = lo.y;
+        h[4 * q + 2] = hi.x;
+        h[4 * q + 3] = hi.y;
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_tile(float *tile, int dim, int d, const float (&h)[N]) {
+#pragma unroll
+    for (int q = 0; q < N / 4; ++q) {
+        f32x2 *p = reinterpret_cast<f32x2 *>(tile + ((size_t)q * dim + d) * 4);
+        p[0] = f32x2{h[4 * q], h[4 * q + 1]};
+        p[1] = f32x2{h[4 * q + 2], h[4 * q + 3]};
+    }
+}
+
+// One wave walks 64 channels of one segment; lane = channel, all N states of it in registers.
+// LOCAL: from zero, gives the segment's end and its sum of delta.  Otherwise: the outputs.
+template <typename DT, int N, bool LOCAL>
+__global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, const ScanGeom g) {
+    typedef typename DT::elem E;
+    const int lane = threadIdx.x;
+    const int group = blockIdx.x % g.groups;
+    const int rest = blockIdx.x / g.groups;
+    const int seg = rest % g.segments, b = rest / g.segments;
+    const int d0 = group * kWave + lane;
+    const bool ok = d0 < a.dim;
+    const int d = ok ? d0 : a.dim - 1;
+    const int t0 = seg * g.seg_len;
+    const int t1 = t0 + g.seg_len < a.length ? t0 + g.seg_len : a.length;
+    const int len = clamp_len(a.lengths, b, a.length);
+    const int te = len < t1 ? (len > t0 ? len : t0) : t1;  // steps of this segment: [t0, te)
+
+    float A2[N], h[N];
+    load_rates<N>(a.A, d, A2);
+    const float bias = a.dt_bias ? a.dt_bias[d] : 0.f;
+    float *seg_state = g.segments > 1 ? g.seg_state + ((size_t)b * g.segments + seg) * N * a.dim : nullptr;
+#pragma unroll
+    for (int n = 0; n < N; ++n) h[n] = 0.f;
+    if (!LOCAL) {
+        if (seg_state) {
+            load_tile<N>(seg_state, a.dim, d, h);
+        } else if (a.initial_state) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) h[n] = a.initial_state[((size_t)b * a.dim + d) * N + n];
+        }
+    }
+    const float skip = !LOCAL && a.D ? a.D[d] : 0.f;
+    const E *xp = static_cast<const E *>(a.x) + b * a.x_batch + d;
+    const E *dtp = static_cast<const E *>(a.dt) + b * a.dt_batch + d;
+    const E *zp = a.z && !LOCAL ? static_cast<const E *>(a.z) + b * a.z_batch + d : nullptr;
+    const E *Bp = static_cast<const E *>(a.B) + b * a.B_batch;
+    const E *Cp = static_cast<const E *>(a.C) + b * a.C_batch;
+    E *yp = LOCAL ? nullptr : static_cast<E *>(a.y) + (size_t)b * a.length * a.dim + d;
+    const int chunks = (a.length + kChunk - 1) / kChunk;
+    float sum_delta = 0.f;
+
+    E xn[kAhead], dtn[kAhead], zn[kAhead];
+    auto fetch = [&](int t) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const long long tt = t + j < te ? t + j : te - 1;
+            xn[j] = xp[tt * a.x_time];
+            dtn[j] = dtp[tt * a.dt_time];
+            if (!LOCAL && zp) zn[j] = zp[tt * a.z_time];
+        }
+    };
+    if (te > t0) fetch(t0);
+    for (int tb = t0; tb < te; tb += kAhead) {
+        E xc[kAhead], dtc[kAhead], zc[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            xc[j] = xn[j];
+            dtc[j] = dtn[j];
+            if (!LOCAL) zc[j] = zn[j];
+        }
+        if (!LOCAL && a.chunk_states && tb % kChunk == 0 && ok)
+            store_tile<N>(a.chunk_states + ((size_t)b * chunks + tb / kChunk) * N * a.dim, a.dim, d, h);
+        fetch(tb + kAhead);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int t = tb + j;
+            if (t >= te) break;
+            ScalarRow<DT, N> B, C;
+            B.load(Bp + t * a.B_time);
+            if (!LOCAL) C.load(Cp + t * a.C_time);
+            float sig;
+            const float x = DT::to_float(xc[j]);
+            const float delta = softplus_(DT::to_float(dtc[j]) + bias, sig);
+            const float dx = delta * x;
+            float y0 = 0.f, y1 = 0.f;  // (two chains)
+#pragma unroll
+            for (int n = 0; n < N; n += 2) {
+                h[n] = fma_(exp2_(delta * A2[n]), h[n], dx * B[n]);
+                h[n + 1] = fma_(exp2_(delta * A2[n + 1]), h[n + 1], dx * B[n + 1]);
+                if (!LOCAL) {
+                    y0 = fma_(C[n], h[n], y0);
+                    y1 = fma_(C[n + 1], h[n + 1], y1);
+                }
+            }
+            if (LOCAL) {
+                sum_delta += delta;
+            } else {
+                float y = fma_(skip, x, y0 + y1);
+                if (zp) {
+                    const float z = DT::to_float(zc[j]);
+                    y *= z * sigmoid_(z);
+                }
+                if (ok) yp[(size_t)t * a.dim] = DT::from_float(y);
+            }
+        }
+    }
+    if (LOCAL) {
+        if (ok) {
+            store_tile<N>(seg_state, a.dim, d, h);
+            g.seg_delta[((size_t)b * g.segments + seg) * a.dim + d] = sum_delta;
+        }
+        return;
+    }
+    if (ok) {
+        for (int t = te; t < t1; ++t) yp[(size_t)t * a.dim] = DT::from_float(0.f);
+        // the segment that holds the last step (segment 0 of an empty sequence) has the final state
+        const bool last = len > t0 ? len <= t1 : (seg == 0 && len == 0);
+        if (a.final_state && last) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) a.final_state[((size_t)b * a.dim + d) * N + n] = h[n];
+        }
+    }
+}
+
+// Pass 2: the state (forward) or the state's gradient (backward) at every segment's border, in order.
+//   forward:  seg_state[s] <- state before segment s;      state <- exp(A sum_delta[s]) state + end[s]
+//   backward: seg_state[s] <- gradient after segment s;    the same towards smaller s, the start grad_final
+// One thread per (sequence, channel, 4 states).
+template <int N, bool BACKWARD>
+__global__ __launch_bounds__(256) void scan_join_kernel(const rnntScan a, const ScanGeom g) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int d = (int)(i % a.dim);
+    const long long r = i / a.dim;
+    const int q = (int)(r % (N / 4));
+    const long long b = r / (N / 4);
+    if (b >= a.batch) return;
+    float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
+    const float *from = BACKWARD ? a.grad_final : a.initial_state;
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        A2[n] = a.A[(size_t)d * N + q * 4 + n] * kLog2e;
+        if (from) h[n] = from[((size_t)b * a.dim + d) * N + q * 4 + n];
+    }
+    for (int k = 0; k < g.segments; ++k) {
+        const int s = BACKWARD ? g.segments - 1 - k : k;
+        float *tile = g.seg_state + (((size_t)b * g.segments + s) * (N / 4) + q) * a.dim * 4 + (size_t)d * 4;
+        const float delta = g.seg_delta[((size_t)b * g.segments + s) * a.dim + d];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const float end = tile[n];
+            tile[n] = h[n];
+            h[n] = fma_(exp2_(delta * A2[n]), h[n], end);
+        }
+    }
+}
+
+// Pass 1 of the backward: the gradient of a segment's first state that its own outputs give.
+//   G <- exp(delta_t A) (G + C_t gy_t), t from the segment's last step to its first
+template <typename DT, int N>
+__global__ __launch_bounds__(64) void scan_backward_local_kernel(const rnntScan a, const ScanGeom g) {
+    typedef typename DT::elem E;
+    const int lane = threadIdx.x;
+    const int group = blockIdx.x % g.groups;
+    const int rest = blockIdx.x / g.groups;
+    const int seg = rest % g.segments, b = rest / g.segments;
+    const int d0 = group * kWave + lane;
+    const bool ok = d0 < a.dim;
+    const int d = ok ? d0 : a.dim - 1;
+    const int t0 = seg * g.seg_len;
+    const int t1 = t0 + g.seg_len < a.length ? t0 + g.seg_len : a.length;
+    const int len = clamp_len(a.lengths, b, a.length);
+    const int te = len < t1 ? (len > t0 ? len : t0) : t1;
+
+    float A2[N], G[N];
+    load_rates<N>(a.A, d, A2);
+#pragma unroll
+    for (int n = 0; n < N; ++n) G[n] = 0.f;
+    const float bias = a.dt_bias ? a.dt_bias[d] : 0.f;
+    const E *dtp = static_cast<const E *>(a.dt) + b * a.dt_batch + d;
+    const E *zp = a.z ? static_cast<const E *>(a.z) + b * a.z_batch + d : nullptr;
+    const E *gp = static_cast<const E *>(a.grad_y) + b * a.grad_y_batch + d;
+    const E *Cp = static_cast<const E *>(a.C) + b * a.C_batch;
+    float sum_delta = 0.f;
+    E dtn[kAhead], zn[kAhead], gn[kAhead];
+    auto fetch = [&](int t) {  // steps t, t - 1, ...
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const long long tt = t - j > t0 ? t - j : t0;
+            dtn[j] = dtp[tt * a.dt_time];
+            gn[j] = gp[tt * a.grad_y_time];
+            if (zp) zn[j] = zp[tt * a.z_time];
+        }
+    };
+    if (te > t0) fetch(te - 1);
+    for (int tb = te - 1; tb >= t0; tb -= kAhead) {
+        E dtc[kAhead], zc[kAhead], gc[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            dtc[j] = dtn[j];
+            gc[j] = gn[j];
+            zc[j] = zn[j];
+        }
+        fetch(tb - kAhead);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int t = tb - j;
+            if (t < t0) break;
+            ScalarRow<DT, N> C;
+            C.load(Cp + t * a.C_time);
+            float sig;
+            const float delta = softplus_(DT::to_float(dtc[j]) + bias, sig);
+            float gy = DT::to_float(gc[j]);
+            if (zp) {
+                const float z = DT::to_float(zc[j]);
+                gy *= z * sigmoid_(z);
+            }
+            sum_delta += delta;
+#pragma unroll
+            for (int n = 0; n < N; ++n) G[n] = exp2_(delta * A2[n]) * fma_(C[n], gy, G[n]);
+        }
+    }
+    if (ok) {
+        store_tile<N>(g.seg_state + ((size_t)b * g.segments + seg) * N * a.dim, a.dim, d, G);
+        g.seg_delta[((size_t)b * g.segments + seg) * a.dim + d] = sum_delta;
+    }
+}
+
+// ---- sums over the 64 lanes of V values at once --------------------------------------------------------------------
+// Every step halves the values and the lanes that share one: 2 V instructions instead of 6 V.  Afterwards lane l holds
+// the sum of value l / (64 / V).
+template <int CTRL>
+__device__ __forceinline__ float dpp_(float v) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int kQuadXor1 = 0xB1, kQuadXor2 = 0x4E, kHalfMirror = 0x141, kRowRor8 = 0x128;
+
+template <int V>
+__device__ __forceinline__ float lanes_sum(float (&v)[V], int lane) {
+    static_assert(V == 4 || V == 8 || V == 16, "");
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + V / 2]), false, false);
+        v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + V / 4]), false, false);
+        v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (V >= 8) {
+        const bool up = lane & 8;
+#pragma unroll
+        for (int i = 0; i < V / 8; ++i) v[i] = (up ? v[i + V / 8] : v[i]) + dpp_<kRowRor8>(up ? v[i] : v[i + V / 8]);
+    } else {
+        v[0] += dpp_<kRowRor8>(v[0]);
+    }
+    if constexpr (V >= 16) {
+        const bool up = lane & 4;
+        v[0] = (up ? v[1] : v[0]) + dpp_<kHalfMirror>(up ? v[0] : v[1]);
+    } else {
+        v[0] += dpp_<kHalfMirror>(v[0]);
+    }
+    v[0] += dpp_<kQuadXor2>(v[0]);
+    v[0] += dpp_<kQuadXor1>(v[0]);
+    return v[0];
+}
+
+// The backward proper.  The N / 4 waves of a workgroup share 64 channels of one segment; wave w owns the states
+// [4 w, 4 w + 4) of all of them, so that a chunk of 16 steps of h and of exp(delta A) stays in registers (2 x 16 x 4)
+// and B, C stay scalar operands.  Per chunk, from the last to the first:
+//   1. each wave turns its share of the steps' inputs into delta, x, gy (LDS), keeping what its outputs need;
+//   2. each wave walks its states forwards from the saved state, then backwards, summing dB, dC over the 64 lanes and
+//      leaving its share of the sums over n in LDS;
+//   3. each wave adds the waves' shares of its steps and writes dx, ddt, dz.
+struct ScanPartials {
+    float *BC;      // [batch][length][groups][2 N]
+    float *A;       // [batch * segments][dim * N]
+    float *D;       // [batch * segments][2][dim]: D, dt_bias
+};
+
+template <typename DT, int N>
+__global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan a, const ScanGeom g, const ScanPartials out) {
+    typedef typename DT::elem E;
+    constexpr int S = 4, W = N / S, kMine = kChunk / W;
+    __shared__ float s_delta[kChunk][kWave], s_x[kChunk][kWave], s_gy[kChunk][kWave];
+    __shared__ float s_part[3][W][kChunk][kWave];
+    __shared__ float s_bc[kChunk][2 * N];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int group = blockIdx.x % g.groups;
+    const int rest = blockIdx.x / g.groups;
+    const int seg = rest % g.segments, b = rest / g.segments;
+    const int d0 = group * kWave + lane;
+    const bool ok = d0 < a.dim;
+    const int d = ok ? d0 : a.dim - 1;
+    const int t0 = seg * g.seg_len;
+    const int t1 = t0 + g.seg_len < a.length ? t0 + g.seg_len : a.length;
+    const int len = clamp_len(a.lengths, b, a.length);
+    const int te = len < t1 ? (len > t0 ? len : t0) : t1;
+    const int chunks = (a.length + kChunk - 1) / kChunk;
+
+    float A2[S], G[S], dA[S];
+#pragma unroll
+    for (int n = 0; n < S; ++n) {
+        A2[n] = a.A[(size_t)d * N + wave * S + n] * kLog2e;
+        G[n] = 0.f;
+        dA[n] = 0.f;
+    }
+    // (states of 4 to a tile row: state n of the layer is element n % 4 of row n / 4)
+    auto tile_at = [&](const float *tile, int n) { return tile + ((size_t)(n / 4) * a.dim + d) * 4 + n % 4; };
+    if (g.segments > 1) {
+        const float *tile = g.seg_state + ((size_t)b * g.segments + seg) * N * a.dim;
+#pragma unroll
+        for (int n = 0; n < S; ++n) G[n] = *tile_at(tile, wave * S + n);
+    } else if (a.grad_final) {
+#pragma unroll
+        for (int n = 0; n < S; ++n) G[n] = a.grad_final[((size_t)b * a.dim + d) * N + wave * S + n];
+    }
+    const float bias = a.dt_bias ? a.dt_bias[d] : 0.f;
+    const float skip = a.D ? a.D[d] : 0.f;
+    const E *xp = static_cast<const E *>(a.x) + b * a.x_batch + d;
+    const E *dtp = static_cast<const E *>(a.dt) + b * a.dt_batch + d;
+    const E *zp = a.z ? static_cast<const E *>(a.z) + b * a.z_batch + d : nullptr;
+    const E *gp = static_cast<const E *>(a.grad_y) + b * a.grad_y_batch + d;
+    const E *Bp = static_cast<const E *>(a.B) + b * a.B_batch + wave * S;
+    const E *Cp = static_cast<const E *>(a.C) + b * a.C_batch + wave * S;
+    const size_t out0 = (size_t)b * a.length * a.dim + d;
+    E *dxp = static_cast<E *>(a.grad_x) + out0, *ddtp = static_cast<E *>(a.grad_dt) + out0;
+    E *dzp = a.z ? static_cast<E *>(a.grad_z) + out0 : nullptr;
+    float dD = 0.f, dbias = 0.f;
+
+    if (ok) {
+        for (int t = te + wave; t < t1; t += W) {
+            dxp[(size_t)t * a.dim] = DT::from_float(0.f);
+            ddtp[(size_t)t * a.dim] = DT::from_float(0.f);
+            if (dzp) dzp[(size_t)t * a.dim] = DT::from_float(0.f);
+        }
+    }
+    for (int c = (te - 1) / kChunk; te > t0 && c >= t0 / kChunk; --c) {
+        const int tc = c * kChunk;
+        float sigv[kMine], dzf[kMine];
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            const int i = wave * kMine + j, t = tc + i;
+            const long long tt = t < te ? t : te - 1;
+            const float x = DT::to_float(xp[tt * a.x_time]);
+            float delta = softplus_(DT::to_float(dtp[tt * a.dt_time]) + bias, sigv[j]);
+            float gy = DT::to_float(gp[tt * a.grad_y_time]);
+            dzf[j] = 0.f;
+            if (zp) {
+                const float z = DT::to_float(zp[tt * a.z_time]), s = sigmoid_(z);
+                dzf[j] = gy * fma_(z * s, 1.f - s, s);
+                gy *= z * s;
+            }
+            const bool in = t < te && ok;  // a step past the end leaves the state and adds nothing
+            s_delta[i][lane] = in ? delta : 0.f;
+            s_x[i][lane] = in ? x : 0.f;
+            s_gy[i][lane] = in ? gy : 0.f;
+        }
+        float h[S];
+        const float *tile = a.chunk_states + ((size_t)b * chunks + c) * N * a.dim;
+#pragma unroll
+        for (int n = 0; n < S; ++n) h[n] = *tile_at(tile, wave * S + n);
+        __syncthreads();
+
+        float before[kChunk][S], decay[kChunk][S];
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) {
+            const long long tt = tc + i < te ? tc + i : te - 1;
+            ScalarRow<DT, S> B, C;
+            B.load(Bp + tt * a.B_time);
+            C.load(Cp + tt * a.C_time);
+            const float delta = s_delta[i][lane], dx = delta * s_x[i][lane];
+            float y = 0.f;
+#pragma unroll
+            for (int n = 0; n < S; ++n) {
+                before[i][n] = h[n];
+                decay[i][n] = exp2_(delta * A2[n]);
+                h[n] = fma_(decay[i][n], h[n], dx * B[n]);
+                y = fma_(C[n], h[n], y);
+            }
+            s_part[0][wave][i][lane] = y;
+        }
+#pragma unroll
+        for (int i = kChunk - 1; i >= 0; --i) {
+            const long long tt = tc + i < te ? tc + i : te - 1;
+            ScalarRow<DT, S> B, C;
+            B.load(Bp + tt * a.B_time);
+            C.load(Cp + tt * a.C_time);
+            const float delta = s_delta[i][lane], dx = delta * s_x[i][lane], gy = s_gy[i][lane];
+            float inner = 0.f, rate = 0.f, sums[2 * S];
+#pragma unroll
+            for (int n = 0; n < S; ++n) {
+                const float after = i + 1 < kChunk ? before[i + 1 < kChunk ? i + 1 : 0][n] : h[n];
+                const float gn = fma_(C[n], gy, G[n]);
+                sums[n] = gn * dx;
+                sums[S + n] = after * gy;
+                inner = fma_(gn, B[n], inner);
+                G[n] = gn * decay[i][n];
+                const float r = G[n] * before[i][n];
+                dA[n] = fma_(r, delta, dA[n]);
+                rate = fma_(r, A2[n], rate);
+            }
+            s_part[1][wave][i][lane] = inner;
+            s_part[2][wave][i][lane] = rate;
+            __builtin_amdgcn_sched_barrier(0);
+            const float sum = lanes_sum<2 * S>(sums, lane);
+            constexpr int kShare = kWave / (2 * S);
+            const int k = lane / kShare;
+            if (lane % kShare == 0) s_bc[i][(k < S ? 0 : N - S) + wave * S + k] = sum;
+        }
+        __syncthreads();
+
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            const int i = wave * kMine + j, t = tc + i;
+            float y = 0.f, inner = 0.f, rate = 0.f;
+#pragma unroll
+            for (int w = 0; w < W; ++w) {
+                y += s_part[0][w][i][lane];
+                inner += s_part[1][w][i][lane];
+                rate += s_part[2][w][i][lane];
+            }
+            const float delta = s_delta[i][lane], x = s_x[i][lane], gy = s_gy[i][lane];
+            if (t < te && ok) {
+                const float ddt = fma_(x, inner, rate * kLn2) * sigv[j];
+                dxp[(size_t)t * a.dim] = DT::from_float(fma_(delta, inner, skip * gy));
+                ddtp[(size_t)t * a.dim] = DT::from_float(ddt);
+                if (dzp) dzp[(size_t)t * a.dim] = DT::from_float(dzf[j] * fma_(skip, x, y));
+                dD = fma_(gy, x, dD);
+                dbias += ddt;
+            }
+        }
+        for (int k = threadIdx.x; k < kChunk * 2 * N; k += W * kWave) {
+            const int i = k / (2 * N), t = tc + i;
+            if (t < te) out.BC[(((size_t)b * a.length + t) * g.groups + group) * 2 * N + k % (2 * N)] = s_bc[i][k % (2 * N)];
+        }
+        __syncthreads();
+    }
+
+    const size_t part = (size_t)b * g.segments + seg;
+    if (ok) {
+#pragma unroll
+        for (int n = 0; n < S; ++n) out.A[(part * a.dim + d) * N + wave * S + n] = dA[n];
+        if (seg == 0 && a.grad_initial) {
+#pragma unroll
+            for (int n = 0; n < S; ++n) a.grad_initial[((size_t)b * a.dim + d) * N + wave * S + n] = G[n];
+        }
+    }
+    s_delta[wave][lane] = dD;
+    s_x[wave][lane] = dbias;
+    __syncthreads();
+    if (wave < 2 && ok) {
+        const float(*v)[kWave] = wave == 0 ? s_delta : s_x;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) sum += v[w][lane];
+        out.D[(part * 2 + wave) * a.dim + d] = sum;
+    }
+}
+
+// dB, dC: the channel groups' shares of every step, in order; dA, dD, ddt_bias: the shares of sequences and segments.
+// Blocks [0, bc_blocks) take the steps, the others the parameters (256 sums each).
+template <typename DT, int N>
+__global__ __launch_bounds__(256) void scan_backward_sum_kernel(const rnntScan a, const ScanGeom g, const ScanPartials in,
+                                                                unsigned bc_blocks) {
+    typedef typename DT::elem E;
+    if (blockIdx.x < bc_blocks) {
+        const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+        const int k = (int)(i % (2 * N));
+        const long long row = i / (2 * N);
+        if (row >= (long long)a.batch * a.length) return;
+        const int b = (int)(row / a.length), t = (int)(row - (long long)b * a.length);
+        float s = 0.f;
+        if (t < clamp_len(a.lengths, b, a.length)) {
+            const float *p = in.BC + (size_t)row * g.groups * 2 * N + k;
+            for (int j = 0; j < g.groups; ++j) s += p[(size_t)j * 2 * N];
+        }
+        E *o = static_cast<E *>(k < N ? a.grad_B : a.grad_C);
+        o[(size_t)row * N + (k < N ? k : k - N)] = DT::from_float(s);
+        return;
+    }
+    const long long i = (long long)(blockIdx.x - bc_blocks) * 256 + threadIdx.x;
+    const int parts = a.batch * g.segments;
+    const long long rates = (long long)a.dim * N;
+    if (i < rates) {
+        float s = 0.f;
+        for (int p = 0; p < parts; ++p) s += in.A[(size_t)p * rates + i];
+        a.grad_A[i] = s;
+    } else if (i < rates + 2 * a.dim) {
+        const long long k = i - rates;
+        float s = 0.f;
+        for (int p = 0; p < parts; ++p) s += in.D[(size_t)p * 2 * a.dim + k];
+        float *o = k < a.dim ? a.grad_D : a.grad_dt_bias;
+        if (o) o[k < a.dim ? k : k - a.dim] = s;
+    }
+}
+
+// One token per sequence: a lane owns 4 states of a channel, N / 4 neighbouring lanes the channel.
+template <typename DT, int N>
+__global__ __launch_bounds__(256) void scan_step_kernel(const rnntScan a) {
+    typedef typename DT::elem E;
+    constexpr int Q = N / 4;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int q = (int)(i % Q);
+    const long long r = i / Q;
+    if (r >= (long long)a.batch * a.dim) return;  // (whole groups of Q lanes)
+    const int b = (int)(r / a.dim), d = (int)(r - (long long)b * a.dim);
+    float sig;
+    const float x = DT::to_float(static_cast<const E *>(a.x)[b * a.x_batch + d]);
+    const float delta = softplus_(DT::to_float(static_cast<const E *>(a.dt)[b * a.dt_batch + d]) + (a.dt_bias ? a.dt_bias[d] : 0.f), sig);
+    const float dx = delta * x;
+    const E *B = static_cast<const E *>(a.B) + b * a.B_batch + q * 4;
+    const E *C = static_cast<const E *>(a.C) + b * a.C_batch + q * 4;
+    const size_t at = (size_t)r * N + q * 4;
+    float y = 0.f, h[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        h[n] = fma_(exp2_(delta * (a.A[(size_t)d * N + q * 4 + n] * kLog2e)), a.initial_state[at + n], dx * DT::to_float(B[n]));
+        y = fma_(DT::to_float(C[n]), h[n], y);
+    }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) a.final_state[at + n] = h[n];
+    if (Q >= 2) y += dpp_<kQuadXor1>(y);
+    if (Q >= 4) y += dpp_<kQuadXor2>(y);
+    if (Q >= 8) y += dpp_<kHalfMirror>(y);
+    if (q == 0) {
+        y = fma_(a.D ? a.D[d] : 0.f, x, y);
+        if (a.z) {
+            const float z = DT::to_float(static_cast<const E *>(a.z)[b * a.z_batch + d]);
+            y *= z * sigmoid_(z);
+        }
+        static_cast<E *>(a.y)[r] = DT::from_float(y);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// causal convolution
+// ---------------------------------------------------------------------------------------------
+constexpr int kRun = 32;  // steps a thread walks
+
+// row t of xe - (W - 1) rows: x for t >= 0, the initial state (zeros) before
+template <typename DT, int W>
+__device__ __forceinline__ float conv_in(const rnntConv &c, int b, long long t, int d) {
+    typedef typename DT::elem E;
+    if (t >= 0) return DT::to_float(static_cast<const E *>(c.x)[b * c.x_batch + t * c.x_time + d]);
+    return c.initial_state ? DT::to_float(static_cast<const E *>(c.initial_state)[((size_t)b * (W - 1) + (W - 1 + t)) * c.dim + d]) : 0.f;
+}
+
+template <typename DT, int W>
+__global__ __launch_bounds__(256) void conv_forward_kernel(const rnntConv c, int runs, int blocks_d) {
+    typedef typename DT::elem E;
+    const int d = (int)(blockIdx.x % blocks_d) * 256 + threadIdx.x;
+    const int rest = blockIdx.x / blocks_d;
+    const int run = rest % runs, b = rest / runs;
+    if (d >= c.dim) return;
+    const int len = clamp_len(c.lengths, b, c.length);
+    const int t0 = run * kRun, t1 = t0 + kRun < c.length ? t0 + kRun : c.length;
+    const int te = len < t1 ? (len > t0 ? len : t0) : t1;
+    float w[W], win[W];
+#pragma unroll
+    for (int k = 0; k < W; ++k) w[k] = c.weight[(size_t)d * W + k];
+    const float bias = c.bias ? c.bias[d] : 0.f;
+    E *y = static_cast<E *>(c.y) + (size_t)b * c.length * c.dim + d;
+    if (te > t0) {
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) win[k + 1] = conv_in<DT, W>(c, b, (long long)t0 - (W - 1) + k, d);
+    }
+    for (int t = t0; t < te; ++t) {
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) win[k] = win[k + 1];
+        win[W - 1] = conv_in<DT, W>(c, b, t, d);
+        float p = bias;
+#pragma unroll
+        for (int k = 0; k < W; ++k) p = fma_(w[k], win[k], p);
+        y[(size_t)t * c.dim] = DT::from_float(c.silu ? p * sigmoid_(p) : p);
+    }
+    for (int t = te; t < t1; ++t) y[(size_t)t * c.dim] = DT::from_float(0.f);
+    if (run == 0 && c.final_state) {
+        float fin[W - 1];  // (all read before any is written: final_state may be the buffer of initial_state)
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) fin[k] = conv_in<DT, W>(c, b, (long long)len - (W - 1) + k, d);
+        E *f = static_cast<E *>(c.final_state) + (size_t)b * (W - 1) * c.dim + d;
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) f[(size_t)k * c.dim] = DT::from_float(fin[k]);
+    }
+}
+
+// dxe[e] = sum_k w[k] gp[e - k] + grad_final, dw[k] = sum_t gp[t] xe[t + k], db = sum gp, with gp = grad_y silu'(p):
+// p is formed again from the W rows that the window holds.  partial: [batch * runs][W + 1][dim].
+template <typename DT, int W>
+__global__ __launch_bounds__(256) void conv_backward_kernel(const rnntConv c, int runs, int blocks_d, float *partial) {
+    typedef typename DT::elem E;
+    const int d = (int)(blockIdx.x % blocks_d) * 256 + threadIdx.x;
+    const int rest = blockIdx.x / blocks_d;
+    const int run = rest % runs, b = rest / runs;
+    if (d >= c.dim) return;
+    const int len = clamp_len(c.lengths, b, c.length);
+    const int t0 = run * kRun, t1 = t0 + kRun < c.length ? t0 + kRun : c.length;
+    float w[W], win[W], gp[W], dw[W], db = 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+        w[k] = c.weight[(size_t)d * W + k];
+        dw[k] = 0.f;
+        gp[k] = 0.f;
+        win[k] = 0.f;
+    }
+    const float bias = c.bias ? c.bias[d] : 0.f;
+    const E *gy = static_cast<const E *>(c.grad_y) + b * c.grad_y_batch + d;
+    E *dx = static_cast<E *>(c.grad_x) + (size_t)b * c.length * c.dim + d;
+    E *di = c.grad_initial ? static_cast<E *>(c.grad_initial) + (size_t)b * (W - 1) * c.dim + d : nullptr;
+    const E *gf = c.grad_final ? static_cast<const E *>(c.grad_final) + (size_t)b * (W - 1) * c.dim + d : nullptr;
+    // rows of dxe that this run writes: its own steps' x rows t0 .. t1-1 and, run 0, the W - 1 rows of the initial state
+    const int first = run == 0 ? -(W - 1) : t0;
+    if (first < len) {
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) win[k + 1] = first - (W - 1) + k >= -(W - 1) ? conv_in<DT, W>(c, b, (long long)first - (W - 1) + k, d) : 0.f;
+    }
+    // gp index: gp[k] = gp at step s - (W - 1) + k, where s is the newest step formed
+    for (int s = first; s < t1 + W - 1; ++s) {
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) {
+            win[k] = win[k + 1];
+            gp[k] = gp[k + 1];
+        }
+        gp[W - 1] = 0.f;
+        win[W - 1] = s < len ? conv_in<DT, W>(c, b, s, d) : 0.f;
+        if (s >= 0 && s < len) {
+            float p = bias;
+#pragma unroll
+            for (int k = 0; k < W; ++k) p = fma_(w[k], win[k], p);
+            float v = DT::to_float(gy[s * c.grad_y_time]);
+            if (c.silu) {
+                const float sg = sigmoid_(p);
+                v *= fma_(p * sg, 1.f - sg, sg);
+            }
+            gp[W - 1] = v;
+            if (s < t1) {  // (steps past t1 belong to the next run)
+                db += v;
+#pragma unroll
+                for (int k = 0; k < W; ++k) dw[k] = fma_(v, win[k], dw[k]);
+            }
+        }
+        const int t = s - (W - 1);  // row whose W steps t .. s are now in gp[0 .. W-1]
+        if (t < first) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) v = fma_(w[W - 1 - k], gp[k], v);
+        if (gf && t >= len - (W - 1) && t < len) v += DT::to_float(gf[(size_t)(t - (len - (W - 1))) * c.dim]);
+        if (t >= 0) {
+            dx[(size_t)t * c.dim] = DT::from_float(t < len ? v : 0.f);
+        } else if (di) {
+            di[(size_t)(t + W - 1) * c.dim] = DT::from_float(v);
+        }
+    }
+    float *o = partial + (size_t)(b * runs + run) * (W + 1) * c.dim + d;
+#pragma unroll
+    for (int k = 0; k < W; ++k) o[(size_t)k * c.dim] = dw[k];
+    o[(size_t)W * c.dim] = db;
+}
+
+template <int W>
+__global__ __launch_bounds__(256) void conv_backward_sum_kernel(const rnntConv c, const float *partial, int parts) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i >= (W + 1) * c.dim) return;
+    float s = 0.f;
+    for (int p = 0; p < parts; ++p) s += partial[(size_t)p * (W + 1) * c.dim + i];
+    const int k = i / c.dim, d = i - k * c.dim;
+    if (k < W)
+        c.grad_weight[(size_t)d * W + k] = s;
+    else if (c.grad_bias)
+        c.grad_bias[d] = s;
+}
+
+template <typename DT, int W>
+__global__ __launch_bounds__(256) void conv_step_kernel(const rnntConv c) {
+    typedef typename DT::elem E;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (long long)c.batch * c.dim) return;
+    const int b = (int)(i / c.dim), d = (int)(i - (long long)b * c.dim);
+    const E *state = static_cast<const E *>(c.initial_state) + (size_t)b * (W - 1) * c.dim + d;
+    E *out = static_cast<E *>(c.final_state) + (size_t)b * (W - 1) * c.dim + d;
+    E win[W];
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) win[k] = state[(size_t)k * c.dim];
+    win[W - 1] = static_cast<const E *>(c.x)[b * c.x_batch + d];
+    float p = c.bias ? c.bias[d] : 0.f;
+#pragma unroll
+    for (int k = 0; k < W; ++k) p = fma_(c.weight[(size_t)d * W + k], DT::to_float(win[k]), p);
+    static_cast<E *>(c.y)[i] = DT::from_float(c.silu ? p * sigmoid_(p) : p);
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) out[(size_t)k * c.dim] = win[k + 1];
+}
+
+// ---------------------------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------------------------
+inline rnntStatus_t launched() { return hipGetLastError() == hipSuccess ? RNNT_STATUS_SUCCESS : RNNT_STATUS_EXECUTION_FAILED; }
+
+inline size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
+
+inline int groups_of(int dim) { return (dim + kWave - 1) / kWave; }
+
+inline bool scan_shape_ok(int batch, int length, int dim, int state) {
+    return batch >= 1 && length >= 1 && dim >= 1 && (state == 8 || state == 16 || state == 32) && length <= (1 << 30) &&
+           (long long)batch * length < (1ll << 31) && (long long)batch * dim * state < (1ll << 31) &&
+           (long long)batch * groups_of(dim) * ((length + kChunk - 1) / kChunk) < (1ll << 31);
+}
+
+// Segments: none while the (sequence, 64 channels) pairs alone fill the chip.
+inline ScanGeom scan_geometry(int batch, int length, int dim) {
+    ScanGeom g = {};
+    g.groups = groups_of(dim);
+    const long long waves = (long long)batch * g.groups;
+    long long want = waves >= 1024 ? 1 : (2048 + waves - 1) / waves;
+    int len = (int)((length + want - 1) / want);
+    if (len < 64) len = 64;
+    g.seg_len = (len + kChunk - 1) / kChunk * kChunk;
+    g.segments = (length + g.seg_len - 1) / g.seg_len;
+    return g;
+}
+
+struct ScanSpace {
+    size_t seg_state, seg_delta, BC, A, D, total;
+};
+inline ScanSpace scan_space(const ScanGeom &g, int batch, int length, int dim, int state, bool backward) {
+    ScanSpace s = {};
+    size_t at = 0;
+    auto take = [&at](size_t floats) {
+        const size_t here = at;
+        at += round16(floats * sizeof(float));
+        return here;
+    };
+    if (g.segments > 1) {
+        s.seg_state = take((size_t)batch * g.segments * state * dim);
+        s.seg_delta = take((size_t)batch * g.segments * dim);
+    }
+    if (backward) {
+        s.BC = take((size_t)batch * length * g.groups * 2 * state);
+        s.A = take((size_t)batch * g.segments * dim * state);
+        s.D = take((size_t)batch * g.segments * 2 * dim);
+    }
+    s.total = at;
+    return s;
+}
+
+inline bool scan_args_ok(const rnntScan *a) {
+    return a != nullptr && a->x && a->dt && a->A && a->B && a->C && scan_shape_ok(a->batch, a->length, a->dim, a->state);
+}
+
+template <int N, bool BACKWARD>
+void launch_join(const rnntScan &a, const ScanGeom &g, hipStream_t st) {
+    const long long n = (long long)a.batch * a.dim * (N / 4);
+    hipLaunchKernelGGL((scan_join_kernel<N, BACKWARD>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a, g);
+}
+
+template <typename DT, int N>
+rnntStatus_t scan_forward(const rnntScan &a, hipStream_t st) {
+    ScanGeom g = scan_geometry(a.batch, a.length, a.dim);
+    const unsigned grid = (unsigned)((long long)a.batch * g.segments * g.groups);
+    if (g.segments > 1) {
+        const ScanSpace s = scan_space(g, a.batch, a.length, a.dim, N, false);
+        if (a.workspace == nullptr || !aligned16(a.workspace)) return RNNT_STATUS_INVALID_VALUE;
+        g.seg_state = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + s.seg_state);
+        g.seg_delta = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + s.seg_delta);
+        hipLaunchKernelGGL((scan_forward_kernel<DT, N, true>), dim3(grid), dim3(64), 0, st, a, g);
+        launch_join<N, false>(a, g, st);
+    }
+    hipLaunchKernelGGL((scan_forward_kernel<DT, N, false>), dim3(grid), dim3(64), 0, st, a, g);
+    return launched();
+}
+
+template <typename DT, int N>
+rnntStatus_t scan_backward(const rnntScan &a, hipStream_t st) {
+    ScanGeom g = scan_geometry(a.batch, a.length, a.dim);
+    const ScanSpace s = scan_space(g, a.batch, a.length, a.dim, N, true);
+    char *ws = static_cast<char *>(a.workspace);
+    const unsigned grid = (unsigned)((long long)a.batch * g.segments * g.groups);
+    if (g.segments > 1) {
+        g.seg_state = reinterpret_cast<float *>(ws + s.seg_state);
+        g.seg_delta = reinterpret_cast<float *>(ws + s.seg_delta);
+        hipLaunchKernelGGL((scan_backward_local_kernel<DT, N>), dim3(grid), dim3(64), 0, st, a, g);
+        launch_join<N, true>(a, g, st);
+    }
+    const ScanPartials p = {reinterpret_cast<float *>(ws + s.BC), reinterpret_cast<float *>(ws + s.A),
+                            reinterpret_cast<float *>(ws + s.D)};
+    hipLaunchKernelGGL((scan_backward_kernel<DT, N>), dim3(grid), dim3(N * 16), 0, st, a, g, p);
+    const unsigned bc = (unsigned)(((long long)a.batch * a.length * 2 * N + 255) / 256);
+    const unsigned pa = (unsigned)(((long long)a.dim * (N + 2) + 255) / 256);
+    hipLaunchKernelGGL((scan_backward_sum_kernel<DT, N>), dim3(bc + pa), dim3(256), 0, st, a, g, p, bc);
+    return launched();
+}
+
+template <typename DT, int N>
+rnntStatus_t scan_step(const rnntScan &a, hipStream_t st) {
+    const long long n = (long long)a.batch * a.dim * (N / 4);
+    hipLaunchKernelGGL((scan_step_kernel<DT, N>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    return launched();
+}
+
+#define SCAN_BY_STATE(FN, DT)                          \
+    switch (a.state) {                                 \
+        case 8: return FN<DT, 8>(a, st);               \
+        case 16: return FN<DT, 16>(a, st);             \
+        case 32: return FN<DT, 32>(a, st);             \
+        default: return RNNT_STATUS_INVALID_VALUE;     \
+    }
+#define SCAN_DISPATCH(FN)                                                      \
+    do {                                                                       \
+        const rnntScan &a = *scan;                                             \
+        hipStream_t st = static_cast<hipStream_t>(scan->stream);               \
+        switch (a.dtype) {                                                     \
+            case RNNT_DTYPE_F32: SCAN_BY_STATE(FN, F32)                        \
+            case RNNT_DTYPE_BF16: SCAN_BY_STATE(FN, BF16)                      \
+            case RNNT_DTYPE_F16: SCAN_BY_STATE(FN, F16)                        \
+            default: return RNNT_STATUS_INVALID_VALUE;                         \
+        }                                                                      \
+    } while (0)
+
+inline int runs_of(int length) { return (length + kRun - 1) / kRun; }
+
+inline bool conv_shape_ok(int batch, int length, int dim, int width) {
+    return batch >= 1 && length >= 1 && dim >= 1 && width >= 2 && width <= 4 && length <= (1 << 30) &&
+           (long long)batch * length < (1ll << 31) && (long long)batch * dim < (1ll << 31) &&
+           (long long)dim * 8 < (1ll << 31) && (long long)batch * runs_of(length) * ((dim + 255) / 256) < (1ll << 31);
+}
+
+template <typename DT, int W>
+rnntStatus_t conv_forward(const rnntConv &c, hipStream_t st) {
+    const int runs = runs_of(c.length), blocks = (c.dim + 255) / 256;
+    hipLaunchKernelGGL((conv_forward_kernel<DT, W>), dim3((unsigned)((long long)c.batch * runs * blocks)), dim3(256), 0, st, c,
+                       runs, blocks);
+    return launched();
+}
+template <typename DT, int W>
+rnntStatus_t conv_backward(const rnntConv &c, hipStream_t st) {
+    const int runs = runs_of(c.length), blocks = (c.dim + 255) / 256;
+    float *partial = static_cast<float *>(c.workspace);
+    hipLaunchKernelGGL((conv_backward_kernel<DT, W>), dim3((unsigned)((long long)c.batch * runs * blocks)), dim3(256), 0, st, c,
+                       runs, blocks, partial);
+    hipLaunchKernelGGL((conv_backward_sum_kernel<W>), dim3((unsigned)(((W + 1) * c.dim + 255) / 256)), dim3(256), 0, st, c,
+                       static_cast<const float *>(partial), c.batch * runs);
+    return launched();
+}
+template <typename DT, int W>
+rnntStatus_t conv_step(const rnntConv &c, hipStream_t st) {
+    const long long n = (long long)c.batch * c.dim;
+    hipLaunchKernelGGL((conv_step_kernel<DT, W>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, c);
+    return launched();
+}
+
+#define CONV_BY_WIDTH(FN, DT)                          \
+    switch (c.width) {                                 \
+        case 2: return FN<DT, 2>(c, st);               \
+        case 3: return FN<DT, 3>(c, st);               \
+        case 4: return FN<DT, 4>(c, st);               \
+        default: return RNNT_STATUS_INVALID_VALUE;     \
+    }
+#define CONV_DISPATCH(FN)                                                      \
+    do {                                                                       \
+        const rnntConv &c = *conv;                                             \
+        hipStream_t st = static_cast<hipStream_t>(conv->stream);               \
+        switch (c.dtype) {                                                     \
+            case RNNT_DTYPE_F32: CONV_BY_WIDTH(FN, F32)                        \
+            case RNNT_DTYPE_BF16: CONV_BY_WIDTH(FN, BF16)                      \
+            case RNNT_DTYPE_F16: CONV_BY_WIDTH(FN, F16)                        \
+            default: return RNNT_STATUS_INVALID_VALUE;                         \
+        }                                                                      \
+    } while (0)
+
+}  // namespace
+
+extern "C" {
+
+rnntStatus_t rnnt_selective_scan_states_size(int batch, int length, int dim, int state, size_t *size_bytes) {
+    if (size_bytes == nullptr || !scan_shape_ok(batch, length, dim, state)) return RNNT_STATUS_INVALID_VALUE;
+    *size_bytes = (size_t)batch * ((length + kChunk - 1) / kChunk) * dim * state * sizeof(float);
+    return RNNT_STATUS_SUCCESS;
+}
+
+rnntStatus_t rnnt_selective_scan_workspace_size(int batch, int length, int dim, int state, int backward, size_t *size_bytes) {
+    if (size_bytes == nullptr || !scan_shape_ok(batch, length, dim, state)) return RNNT_STATUS_INVALID_VALUE;
+    *size_bytes = scan_space(scan_geometry(batch, length, dim), batch, length, dim, state, backward != 0).total;
+    return RNNT_STATUS_SUCCESS;
+}
+
+rnntStatus_t rnnt_selective_scan_forward(const rnntScan *scan) {
+    if (!scan_args_ok(scan) || scan->y == nullptr || (scan->chunk_states && !aligned16(scan->chunk_states)))
+        return RNNT_STATUS_INVALID_VALUE;
+    SCAN_DISPATCH(scan_forward);
+}
+
+rnntStatus_t rnnt_selective_scan_backward(const rnntScan *scan) {
+    if (!scan_args_ok(scan) || !scan->grad_y || !scan->chunk_states || !aligned16(scan->chunk_states) || !scan->grad_x ||
+        !scan->grad_dt || !scan->grad_A || !scan->grad_B || !scan->grad_C || (scan->z == nullptr) != (scan->grad_z == nullptr) ||
+        !scan->workspace || !aligned16(scan->workspace))
+        return RNNT_STATUS_INVALID_VALUE;
+    SCAN_DISPATCH(scan_backward);
+}
+
+rnntStatus_t rnnt_selective_scan_step(const rnntScan *scan) {
+    if (scan == nullptr || !scan->x || !scan->dt || !scan->A || !scan->B || !scan->C || !scan->y || !scan->initial_state ||
+        !scan->final_state || !scan_shape_ok(scan->batch, 1, scan->dim, scan->state))
+        return RNNT_STATUS_INVALID_VALUE;
+    SCAN_DISPATCH(scan_step);
+}
+
+rnntStatus_t rnnt_causal_conv_workspace_size(int batch, int length, int dim, int width, size_t *size_bytes) {
+    if (size_bytes == nullptr || !conv_shape_ok(batch, length, dim, width)) return RNNT_STATUS_INVALID_VALUE;
+    *size_bytes = (size_t)batch * runs_of(length) * (width + 1) * dim * sizeof(float);
+    return RNNT_STATUS_SUCCESS;
+}
+
+rnntStatus_t rnnt_causal_conv_forward(const rnntConv *conv) {
+    if (conv == nullptr || !conv->x || !conv->weight || !conv->y ||
+        !conv_shape_ok(conv->batch, conv->length, conv->dim, conv->width))
+        return RNNT_STATUS_INVALID_VALUE;
+    CONV_DISPATCH(conv_forward);
+}
+
+rnntStatus_t rnnt_causal_conv_backward(const rnntConv *conv) {
+    if (conv == nullptr || !conv->x || !conv->weight || !conv->grad_y || !conv->grad_x || !conv->grad_weight || !conv->workspace ||
+        !aligned16(conv->workspace) || !conv_shape_ok(conv->batch, conv->length, conv->dim, conv->width))
+        return RNNT_STATUS_INVALID_VALUE;
+    CONV_DISPATCH(conv_backward);
+}
+
+rnntStatus_t rnnt_causal_conv_step(const rnntConv *conv) {
+    if (conv == nullptr || !conv->x || !conv->weight || !conv->y || !conv->initial_state || !conv->final_state ||
+        !conv_shape_ok(conv->batch, 1, conv->dim, conv->width))
+        return RNNT_STATUS_INVALID_VALUE;
+    CONV_DISPATCH(conv_step);
+}
+
+}  // extern "C"

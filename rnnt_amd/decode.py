@@ -11,19 +11,23 @@ frame), with one host round trip per window or emission instead of one per frame
 """
 from __future__ import annotations
 
-from typing import Callable, List, Tuple
+from typing import Callable, List, Optional, Tuple
 
 import torch
 import torch.nn.functional as F
 
-from . import _lib
+from . import _lib, _torch_binding
 from .joint import JointNet, joint_hidden
+from .rules import HistoryRules, LogitRules, _check
 
 _DTYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16, torch.float16: _lib.DTYPE_F16}
 
 
-def row_argmax(x: torch.Tensor) -> torch.Tensor:
-    """``int32[R]``: first index of the maximum of every row of ``x[R, V]`` (NaN counts as maximum)."""
+def row_argmax(x: torch.Tensor, rules: Optional[LogitRules] = None) -> torch.Tensor:
+    """``int32[R]``: first index of the maximum of every row of ``x[R, V]`` (NaN counts as maximum), of the logits as
+    ``rules`` change them if given (:class:`rnnt_amd.LogitRules`)."""
+    if rules is not None:
+        return _torch_binding.load().row_rules(x, *_check(rules)._args(), False)[0]
     if x.dim() != 2 or x.shape[0] < 1 or x.shape[1] < 1:
         raise ValueError("x must be a non-empty [rows, V] tensor")
     if x.dtype not in _DTYPES:
@@ -38,9 +42,12 @@ def row_argmax(x: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def row_max_logp(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+def row_max_logp(x: torch.Tensor, rules: Optional[LogitRules] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(int32[R], float32[R])``: argmax of every row of ``x[R, V]`` as :func:`row_argmax` gives it, and
-    ``max(log_softmax(row))``, i.e. ``torch.max(F.log_softmax(x, -1), dim=1)`` in one launch."""
+    ``max(log_softmax(row))``, i.e. ``torch.max(F.log_softmax(x, -1), dim=1)`` in one launch; both of the logits as
+    ``rules`` change them if given."""
+    if rules is not None:
+        return _torch_binding.load().row_rules(x, *_check(rules)._args(), True)
     if x.dim() != 2 or x.shape[0] < 1 or x.shape[1] < 1:
         raise ValueError("x must be a non-empty [rows, V] tensor")
     if x.dtype not in _DTYPES:
@@ -66,7 +73,7 @@ def _joint_weights(joint: JointNet, he: int):
 
 @torch.no_grad()
 def greedy_search_batch(encoder_output: torch.Tensor, decoder: Callable, joint: JointNet, blank: int = 0,
-                        window: int = 32):
+                        window: int = 32, rules: Optional[LogitRules] = None):
     """The reference's batched greedy search, ``TransducerBeamSearcher.transducer_greedy_decode``
     (/root/reference/src/rnnt/beam_searcher.py:65-127), with one host round trip per window of frames.
 
@@ -82,7 +89,9 @@ def greedy_search_batch(encoder_output: torch.Tensor, decoder: Callable, joint: 
         encoder_output: ``[B, T, He]``; as in the reference all ``T`` frames of every utterance are decoded.
         decoder: called as the reference calls it: ``decoder(tokens[n,1])`` and
             ``decoder(tokens[n,1], hidden=hidden)`` -> ``(out[n,1,Hd], hidden)``, hidden a tensor or an
-            ``(h, c)`` tuple shaped ``[layers, n, Hd]``.
+            ``(h, c)`` tuple shaped ``[layers, n, Hd]`` (or ``[layers, n, ...]``: :class:`rnnt_amd.PredictionNet`).
+        rules: penalties, biases and masks on the logits (:class:`rnnt_amd.LogitRules`); an utterance's history is what it
+            has emitted, after ``rules.history`` if given.  A mask has to allow ``blank`` wherever no emission is due.
     Returns:
         ``(predictions, mean(exp(score)), None, None)`` as the reference's 4-tuple (``:122-127``): token lists
         per utterance, and the batch mean of ``exp`` of each utterance's summed log-probabilities of its
@@ -104,6 +113,7 @@ def greedy_search_batch(encoder_output: torch.Tensor, decoder: Callable, joint: 
     dec_proj = F.linear(out_pn, w_dec)                                          # [B, 1, H]
     ptr = [0] * B
     offs = torch.arange(window, device=dev)
+    kept = None if rules is None else HistoryRules(rules, B, out.out_features, T, dev)
     while True:
         active = [b for b in range(B) if ptr[b] < T]
         if not active:
@@ -113,7 +123,7 @@ def greedy_search_batch(encoder_output: torch.Tensor, decoder: Callable, joint: 
         frames = torch.clamp(start[:, None] + offs[None, :], max=T - 1)         # [A, W]; surplus frames ignored below
         win = enc_proj[act[:, None], frames]                                    # [A, W, H]
         h = joint_hidden(win.contiguous(), dec_proj[act].contiguous())          # [A, W, 1, H]
-        pos, logp = row_max_logp(out(h.reshape(len(active) * window, -1)))
+        pos, logp = row_max_logp(out(h.reshape(len(active) * window, -1)), None if kept is None else kept.of(active))
         host = torch.stack((pos, logp.view(torch.int32))).cpu()                 # the one host round trip
         pos_h = host[0].reshape(len(active), window).tolist()
         logp_h = host[1].view(torch.float32).reshape(len(active), window).tolist()
@@ -129,6 +139,8 @@ def greedy_search_batch(encoder_output: torch.Tensor, decoder: Callable, joint: 
             ptr[b] += step + 1                                                  # one symbol per frame at most
             emitted.append(b)
         if emitted:
+            if kept is not None:
+                kept.emit(emitted, [predictions[b][-1] for b in emitted])
             sel = torch.tensor(emitted, device=dev)
             input_decoder[sel, 0] = torch.tensor([predictions[b][-1] for b in emitted], device=dev)
             if isinstance(hidden, tuple):
@@ -148,7 +160,7 @@ def greedy_search_batch(encoder_output: torch.Tensor, decoder: Callable, joint: 
 
 @torch.no_grad()
 def greedy_decode(enc_state: torch.Tensor, length: int, decoder: Callable, joint: JointNet, blank: int = 0,
-                  window: int = 32) -> List[int]:
+                  window: int = 32, rules: Optional[LogitRules] = None) -> List[int]:
     """Tokens of one utterance, as ``decode(enc_state, lengths)`` of the reference (model.py:145-165).
 
     Args:
@@ -158,6 +170,7 @@ def greedy_decode(enc_state: torch.Tensor, length: int, decoder: Callable, joint
             ``decoder(token[1,1], hidden=hidden)`` -> ``(dec_state[1,1,Hd], hidden)``.
         joint: :class:`rnnt_amd.JointNet` (its two Linear layers are used directly).
         window: frames evaluated per launch.
+        rules: as in :func:`greedy_search_batch`, for the one utterance.
     """
     if enc_state.dim() != 2:
         raise ValueError("enc_state must be [T, He]")
@@ -177,16 +190,19 @@ def greedy_decode(enc_state: torch.Tensor, length: int, decoder: Callable, joint
     zero_token = torch.zeros((1, 1), dtype=torch.long, device=dev)
     dec_state, hidden = decoder(zero_token)
     dec_proj = F.linear(dec_state.reshape(1, 1, -1), w_dec)                  # [1, 1, H]
+    kept = None if rules is None else HistoryRules(rules, 1, out.out_features, length, dev)
     t = 0
     while t < length:
         n = min(window, length - t)
         h = joint_hidden(enc_proj[:, t:t + n].contiguous(), dec_proj)        # [1, n, 1, H]
-        pred = row_argmax(out(h.reshape(n, -1))).tolist()                    # the one host round trip
+        pred = row_argmax(out(h.reshape(n, -1)), None if kept is None else kept.of([0])).tolist()   # the one host round trip
         step = next((i for i, p in enumerate(pred) if p != blank), None)
         if step is None:
             t += n
             continue
         tokens.append(pred[step])
+        if kept is not None:
+            kept.emit([0], [pred[step]])
         dec_state, hidden = decoder(torch.full((1, 1), pred[step], dtype=torch.long, device=dev), hidden=hidden)
         dec_proj = F.linear(dec_state.reshape(1, 1, -1), w_dec)
         t += step + 1                                                        # at most one symbol per frame
