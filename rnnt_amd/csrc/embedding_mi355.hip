@@ -19,9 +19,11 @@ namespace {
 using namespace rnnt_mi355_detail;
 
 constexpr int kBlock = 256;
-constexpr int kPiece = 32;        // sorted positions per piece
+constexpr int kBatch = 8;         // gradient rows loaded at once
 constexpr int kRankMax = 4096;    // up to this many positions are sorted by counting smaller ones
-constexpr int kSortItems = 4096;  // positions per workgroup and pass of the radix sort
+constexpr int kRankRows = 64;     // rows of the gradient that a workgroup of the counting kernel clears
+constexpr int kSortItems = 1024;  // positions per workgroup and pass of the radix sort
+constexpr int kJoinWaves = 8;
 constexpr int kDigits = 256;
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -74,18 +76,70 @@ __global__ __launch_bounds__(kBlock) void embed_forward_kernel(const void *__res
 }
 
 // ---- sorting ---------------------------------------------------------------------------------------------------------
-// Few positions: a position's place is the number of positions before it in the order, counted against all others.
-// n^2 comparisons over n / 256 workgroups in one launch, nothing to wait for.
+// Few positions: a position's place is the number of positions before it in the order, counted against all others:
+// n^2 comparisons in one launch, nothing to wait for.  A workgroup places 64 positions (its lanes), each wave against a
+// quarter of the keys, four keys to an LDS read; "equal and earlier" is decided per block of keys, not per key.
+// The workgroups from rank_blocks on clear 64 rows of the gradient each, those whose token no position holds.
+template <typename DT, int VEC>
 __global__ __launch_bounds__(kBlock) void embed_rank_kernel(const void *__restrict__ tokens, int tokens_64, int n, int vocab,
-                                                            long long padding, int *__restrict__ sorted, int *__restrict__ order) {
-    __shared__ int s_key[kRankMax];
-    for (int j = threadIdx.x; j < n; j += kBlock) s_key[j] = key_at(tokens, tokens_64, j, vocab, padding);
+                                                            long long padding, int *__restrict__ sorted, int *__restrict__ order,
+                                                            typename DT::elem *__restrict__ grad_weight, int dim, int rank_blocks) {
+    typedef int i32x4 __attribute__((ext_vector_type(4)));
+    constexpr int kWaves = kBlock / kWave;
+    __shared__ i32x4 s_key[kRankMax / 4];
+    __shared__ int s_rank[kWaves][kWave];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if ((int)blockIdx.x >= rank_blocks) {
+        const int v0 = ((int)blockIdx.x - rank_blocks) * kRankRows;
+        int *held = &s_rank[0][0];
+        if (threadIdx.x < kRankRows) held[threadIdx.x] = 0;
+        __syncthreads();
+        for (int j = threadIdx.x; j < n; j += kBlock) {
+            const int k = key_at(tokens, tokens_64, j, vocab, padding) - v0;
+            if (k >= 0 && k < kRankRows) held[k] = 1;
+        }
+        __syncthreads();
+        const float zero[VEC] = {};
+        for (int r = wave; r < kRankRows && v0 + r < vocab; r += kWaves) {
+            if (held[r]) continue;
+            for (int c = lane * VEC; c < dim; c += kWave * VEC) store_piece<DT, VEC>(grad_weight + (size_t)(v0 + r) * dim + c, zero);
+        }
+        return;
+    }
+    int *keys = reinterpret_cast<int *>(s_key);
+    const int padded = (n + 3) & ~3;
+    for (int j = threadIdx.x; j < padded; j += kBlock) keys[j] = j < n ? key_at(tokens, tokens_64, j, vocab, padding) : 0x7fffffff;
     __syncthreads();
-    const int i = blockIdx.x * kBlock + threadIdx.x;
-    if (i >= n) return;
-    const int key = s_key[i];
+    const int i0 = blockIdx.x * kWave, i = i0 + lane;
+    const int key = i < n ? keys[i] : 0x7fffffff;
+    const int quads = padded / 4, per = (quads + kWaves - 1) / kWaves;
+    const int q0 = wave * per, q1 = q0 + per < quads ? q0 + per : quads;
+    // quads [q0, qa): before this block of positions, equal keys count; [qa, qb): inside; [qb, q1): after, they do not
+    const int qa = min(max(i0 / 4, q0), q1), qb = min(max((i0 + kWave) / 4, q0), q1);
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += s_key[j] < key || (s_key[j] == key && j < i);
+#pragma unroll 8
+    for (int q = q0; q < qa; ++q) {
+        const i32x4 k = s_key[q];
+        rank += (k.x <= key) + (k.y <= key) + (k.z <= key) + (k.w <= key);
+    }
+    for (int q = qa; q < qb; ++q) {
+        const i32x4 k = s_key[q];
+        const int j = q * 4;
+        rank += (k.x < key || (k.x == key && j < i)) + (k.y < key || (k.y == key && j + 1 < i)) +
+                (k.z < key || (k.z == key && j + 2 < i)) + (k.w < key || (k.w == key && j + 3 < i));
+    }
+#pragma unroll 8
+    for (int q = max(qb, q0); q < q1; ++q) {
+        const i32x4 k = s_key[q];
+        rank += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
+    }
+    s_rank[wave][lane] = rank;
+    __syncthreads();
+    if (wave != 0 || i >= n) return;
+    rank = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) rank += s_rank[w][lane];
     sorted[rank] = key;
     order[rank] = i;
 }
@@ -197,119 +251,139 @@ __device__ __forceinline__ int lower_bound(const int *sorted, int n, int key) {
     return lo;
 }
 
-// Groups [0, pieces): a piece of sorted positions each.  A run of equal tokens inside the piece is written out; the part
-// of a run that began in an earlier piece goes to partial[piece][0], the part of one that begins here and goes on to
-// partial[piece][1].  Groups [pieces, pieces + vocab): the rows of tokens that no position holds are set to zero.
+// Groups of 2^shift lanes.  [0, pieces * slices): a slice of the columns of a piece of sorted positions each.  A run of
+// equal tokens inside the piece is written out; the part of a run that began in an earlier piece goes to
+// partial[piece][0], the part of one that begins here and goes on to partial[piece][1].  Rows are loaded kBatch at a
+// time: a piece is a chain of dependent additions, but its loads are not.
+// The waves behind them (zero_waves of 16 rows) clear the rows that no position holds: a lane searches for each.
 template <typename DT, int VEC>
 __global__ __launch_bounds__(kBlock) void embed_sum_kernel(const int *__restrict__ sorted, const int *__restrict__ order, int n,
                                                            const typename DT::elem *__restrict__ grad, long long grad_stride,
                                                            int vocab, int dim, float scale,
                                                            typename DT::elem *__restrict__ grad_weight,
-                                                           float *__restrict__ partial, int pieces, int shift) {
-    const int sub = threadIdx.x & ((1 << shift) - 1);
-    const long long group = ((long long)blockIdx.x * kBlock + threadIdx.x) >> shift;
-    const int width = VEC << shift;
-    if (group >= pieces) {
-        const long long v = group - pieces;
-        if (v >= vocab) return;
-        const int at = lower_bound(sorted, n, (int)v);
-        if (at < n && sorted[at] == (int)v) return;
+                                                           float *__restrict__ partial, int piece, int pieces, int slices, int shift,
+                                                           unsigned sum_blocks) {
+    if (blockIdx.x >= sum_blocks) {
+        const int lane = threadIdx.x & (kWave - 1);
+        const long long wave = (long long)(blockIdx.x - sum_blocks) * (kBlock / kWave) + threadIdx.x / kWave;
+        const long long v0 = wave * 16;
+        const int v = (int)(v0 + (lane & 15) < vocab ? v0 + (lane & 15) : vocab - 1);
+        const int at = lower_bound(sorted, n, v);
+        const unsigned long long held = __ballot(at < n && sorted[at] == v);
         const float zero[VEC] = {};
-        for (int c = sub * VEC; c < dim; c += width) store_piece<DT, VEC>(grad_weight + (size_t)v * dim + c, zero);
+        for (int r = 0; r < 16 && v0 + r < vocab; ++r) {
+            if (held >> r & 1) continue;
+            for (int c = lane * VEC; c < dim; c += kWave * VEC) store_piece<DT, VEC>(grad_weight + (size_t)(v0 + r) * dim + c, zero);
+        }
         return;
     }
-    const int begin = (int)group * kPiece, end = begin + kPiece < n ? begin + kPiece : n;
+    const int sub = threadIdx.x & ((1 << shift) - 1);
+    const long long group = ((long long)blockIdx.x * kBlock + threadIdx.x) >> shift;
+    const long long p = group / slices;
+    if (p >= pieces) return;
+    const int c = ((int)(group - p * slices) << shift) * VEC + sub * VEC;
+    if (c >= dim) return;
+    const int begin = (int)p * piece, end = begin + piece < n ? begin + piece : n;
     const int prev = begin > 0 ? sorted[begin - 1] : -1, next = end < n ? sorted[end] : -1;
-    for (int c = sub * VEC; c < dim; c += width) {
-        float acc[VEC] = {};
-        int cur = sorted[begin];
-        bool from_before = cur == prev;
-        auto close = [&](bool goes_on) {
-            if (cur == vocab) return;
-            if (from_before || goes_on) {
-                float *p = partial + ((size_t)group * 2 + (from_before ? 0 : 1)) * dim + c;
+    float acc[VEC] = {};
+    int cur = sorted[begin];
+    bool from_before = cur == prev;
+    auto close = [&](bool goes_on) {
+        if (cur == vocab) return;
+        if (from_before || goes_on) {
+            float *o = partial + ((size_t)p * 2 + (from_before ? 0 : 1)) * dim + c;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) p[j] = acc[j];
-            } else {
-                float f[VEC];
+            for (int j = 0; j < VEC; ++j) o[j] = acc[j];
+        } else {
+            float f[VEC];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) f[j] = acc[j] * scale;
-                store_piece<DT, VEC>(grad_weight + (size_t)cur * dim + c, f);
-            }
-        };
-        for (int k = begin; k < end; ++k) {
-            const int tok = sorted[k];
-            if (tok != cur) {
+            for (int j = 0; j < VEC; ++j) f[j] = acc[j] * scale;
+            store_piece<DT, VEC>(grad_weight + (size_t)cur * dim + c, f);
+        }
+    };
+    for (int k0 = begin; k0 < end && cur != vocab; k0 += kBatch) {
+        int tok[kBatch];
+        float f[kBatch][VEC];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const int at = k0 + k < end ? k0 + k : end - 1;
+            tok[k] = sorted[at];
+            load_piece<DT, VEC>(grad + (size_t)order[at] * grad_stride + c, f[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            if (k0 + k >= end || cur == vocab) break;
+            if (tok[k] != cur) {
                 close(false);
-                cur = tok;
+                cur = tok[k];
                 from_before = false;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
             }
-            if (tok == vocab) break;
-            float f[VEC];
-            load_piece<DT, VEC>(grad + (size_t)order[k] * grad_stride + c, f);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[j] += f[j];
+            for (int j = 0; j < VEC; ++j) acc[j] += f[k][j];
         }
-        close(cur == next);
     }
+    close(cur == next);
 }
 
 // The runs that cross pieces: the workgroup of the piece a run begins in adds the run's parts, each wave a range of
-// the pieces in order, then the waves' sums in order.
+// the pieces in order, then the waves' sums in order.  grid.y: slices of 64 VEC columns.
 template <typename DT, int VEC>
-__global__ __launch_bounds__(kBlock) void embed_join_kernel(const int *__restrict__ sorted, int n, int vocab, int dim, float scale,
-                                                            typename DT::elem *__restrict__ grad_weight,
-                                                            const float *__restrict__ partial, int pieces) {
-    constexpr int kWaves = kBlock / kWave;
-    __shared__ float s_acc[kWaves][kWave * VEC];
-    const int piece = blockIdx.x;
-    const int begin = piece * kPiece, end = begin + kPiece;
+__global__ __launch_bounds__(kJoinWaves *kWave) void embed_join_kernel(const int *__restrict__ sorted, int n, int vocab, int dim,
+                                                                       float scale, typename DT::elem *__restrict__ grad_weight,
+                                                                       const float *__restrict__ partial, int piece) {
+    __shared__ float s_acc[kJoinWaves][kWave * VEC];
+    const int p = blockIdx.x;
+    const int begin = p * piece, end = begin + piece;
     if (end >= n) return;
     const int tok = sorted[end - 1];
     if (tok == vocab || sorted[end] != tok) return;
     if (sorted[begin] == tok && begin > 0 && sorted[begin - 1] == tok) return;  // began earlier
-    const int stop = lower_bound(sorted, n, tok + 1);  // end of the run
-    const int last = (stop - 1) / kPiece;              // pieces piece + 1 .. last hold parts of it
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int parts = last - piece, per = (parts + kWaves - 1) / kWaves;
-    const int p0 = piece + 1 + wave * per, p1 = p0 + per < last + 1 ? p0 + per : last + 1;
-    for (int c0 = 0; c0 < dim; c0 += kWave * VEC) {
-        const int c = c0 + lane * VEC;
-        float acc[VEC] = {};
-        if (c < dim) {
-            if (wave == 0) {
+    const int stop = lower_bound(sorted, n, tok + 1);  // end of the run
+    const int last = (stop - 1) / piece;               // pieces p + 1 .. last hold parts of it
+    const int parts = last - p, per = (parts + kJoinWaves - 1) / kJoinWaves;
+    const int p0 = p + 1 + wave * per, p1 = p0 + per < last + 1 ? p0 + per : last + 1;
+    const int c = (int)blockIdx.y * kWave * VEC + lane * VEC;
+    float acc[VEC] = {};
+    if (c < dim) {
+        if (wave == 0) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) acc[j] = partial[((size_t)piece * 2 + 1) * dim + c + j];
-            }
-            for (int p = p0; p < p1; ++p)
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) acc[j] += partial[(size_t)p * 2 * dim + c + j];
+            for (int j = 0; j < VEC; ++j) acc[j] = partial[((size_t)p * 2 + 1) * dim + c + j];
         }
+#pragma unroll 8
+        for (int q = p0; q < p1; ++q) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) s_acc[wave][lane * VEC + j] = acc[j];
-        __syncthreads();
-        if (wave == 0 && c < dim) {
-            float f[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                float s = 0.f;
-#pragma unroll
-                for (int w = 0; w < kWaves; ++w) s += s_acc[w][lane * VEC + j];
-                f[j] = s * scale;
-            }
-            store_piece<DT, VEC>(grad_weight + (size_t)tok * dim + c, f);
+            for (int j = 0; j < VEC; ++j) acc[j] += partial[(size_t)q * 2 * dim + c + j];
         }
-        __syncthreads();
     }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) s_acc[wave][lane * VEC + j] = acc[j];
+    __syncthreads();
+    if (wave != 0 || c >= dim) return;
+    float f[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWaves; ++w) s += s_acc[w][lane * VEC + j];
+        f[j] = s * scale;
+    }
+    store_piece<DT, VEC>(grad_weight + (size_t)tok * dim + c, f);
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
 struct EmbedSpace {
     size_t sorted[2], order[2], counts, partial, total;
 };
-inline int pieces_of(long long n) { return (int)((n + kPiece - 1) / kPiece); }
+// Positions per piece: short pieces while there are few, so that they fill the chip; longer ones keep the joining short.
+inline int piece_of(long long n) {
+    int piece = kBatch;
+    while (piece < 64 && n / piece > 4096) piece *= 2;
+    return piece;
+}
+inline int pieces_of(long long n) { return (int)((n + piece_of(n) - 1) / piece_of(n)); }
 inline int sort_blocks(long long n) { return (int)((n + kSortItems - 1) / kSortItems); }
 inline EmbedSpace embed_space(long long n, int dim) {
     EmbedSpace s = {};
@@ -331,7 +405,7 @@ inline EmbedSpace embed_space(long long n, int dim) {
 }
 
 inline bool embed_shape_ok(long long n, int vocab, int dim) {
-    return n >= 1 && n < (1ll << 31) - (1 << 16) && vocab >= 1 && vocab < 0x7fffffff && dim >= 1 && dim <= (1 << 24);
+    return n >= 1 && n < (1ll << 31) - (1 << 16) && vocab >= 1 && vocab < 0x7fffffff && dim >= 1 && dim <= (1 << 21);
 }
 
 // lanes that share a row: a power of two that covers the row's pieces, at most a wave
@@ -358,10 +432,10 @@ rnntStatus_t embed_forward(const void *tokens, int tokens_64, long long n, const
     return hipGetLastError() == hipSuccess ? RNNT_STATUS_SUCCESS : RNNT_STATUS_EXECUTION_FAILED;
 }
 
-template <typename DT>
-rnntStatus_t embed_backward(const void *tokens, int tokens_64, long long n, const void *grad, long long grad_stride, int vocab,
-                            int dim, float scale, long long padding, void *grad_weight, void *workspace, hipStream_t st) {
-    typedef typename DT::elem E;
+template <typename DT, int VEC>
+rnntStatus_t embed_backward_with(const void *tokens, int tokens_64, int n, const typename DT::elem *grad, long long grad_stride,
+                                 int vocab, int dim, float scale, long long padding, typename DT::elem *grad_weight, void *workspace,
+                                 hipStream_t st) {
     const EmbedSpace sp = embed_space(n, dim);
     char *ws = static_cast<char *>(workspace);
     int *sorted[2], *order[2];
@@ -372,45 +446,47 @@ rnntStatus_t embed_backward(const void *tokens, int tokens_64, long long n, cons
     float *partial = reinterpret_cast<float *>(ws + sp.partial);
     int at = 0;
     if (n <= kRankMax) {
-        hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)((n + kBlock - 1) / kBlock)), dim3(kBlock), 0, st, tokens, tokens_64,
-                           (int)n, vocab, padding, sorted[0], order[0]);
+        const int blocks = (n + kWave - 1) / kWave;
+        hipLaunchKernelGGL((embed_rank_kernel<DT, VEC>), dim3(blocks + (vocab - 1) / kRankRows + 1), dim3(kBlock), 0, st, tokens, tokens_64,
+                           n, vocab, padding, sorted[0], order[0], grad_weight, dim, blocks);
     } else {
         int *counts = reinterpret_cast<int *>(ws + sp.counts);
         const dim3 grid((unsigned)sort_blocks(n));
-        hipLaunchKernelGGL((embed_digit_kernel<true>), grid, dim3(kBlock), 0, st, tokens, tokens_64, (int)n, vocab, padding, 0, counts);
-        hipLaunchKernelGGL((embed_place_kernel<true>), grid, dim3(kBlock), 0, st, tokens, tokens_64, (int)n, vocab, padding, 0,
+        hipLaunchKernelGGL((embed_digit_kernel<true>), grid, dim3(kBlock), 0, st, tokens, tokens_64, n, vocab, padding, 0, counts);
+        hipLaunchKernelGGL((embed_place_kernel<true>), grid, dim3(kBlock), 0, st, tokens, tokens_64, n, vocab, padding, 0,
                            static_cast<const int *>(counts), static_cast<const int *>(nullptr), sorted[0], order[0]);
         for (int bit = 8; bit < 31 && (vocab >> bit) != 0; bit += 8) {
-            hipLaunchKernelGGL((embed_digit_kernel<false>), grid, dim3(kBlock), 0, st, static_cast<const void *>(sorted[at]), 0, (int)n,
-                               vocab, padding, bit, counts);
-            hipLaunchKernelGGL((embed_place_kernel<false>), grid, dim3(kBlock), 0, st, static_cast<const void *>(sorted[at]), 0, (int)n,
-                               vocab, padding, bit, static_cast<const int *>(counts), static_cast<const int *>(order[at]),
-                               sorted[1 - at], order[1 - at]);
+            hipLaunchKernelGGL((embed_digit_kernel<false>), grid, dim3(kBlock), 0, st, static_cast<const void *>(sorted[at]), 0, n, vocab,
+                               padding, bit, counts);
+            hipLaunchKernelGGL((embed_place_kernel<false>), grid, dim3(kBlock), 0, st, static_cast<const void *>(sorted[at]), 0, n, vocab,
+                               padding, bit, static_cast<const int *>(counts), static_cast<const int *>(order[at]), sorted[1 - at],
+                               order[1 - at]);
             at = 1 - at;
         }
     }
-    const bool vec = dim % DT::EPC == 0 && grad_stride % DT::EPC == 0 && aligned16(grad) && aligned16(grad_weight);
-    const int shift = row_shift(dim, vec ? DT::EPC : 1);
-    const int pieces = pieces_of(n);
-    const long long blocks = ((((long long)pieces + vocab) << shift) + kBlock - 1) / kBlock;
-    if (blocks > 0x7fffffffll) return RNNT_STATUS_INVALID_VALUE;
-#define EMBED_SUM(VEC)                                                                                                       \
-    do {                                                                                                                     \
-        hipLaunchKernelGGL((embed_sum_kernel<DT, VEC>), dim3((unsigned)blocks), dim3(kBlock), 0, st,                         \
-                           static_cast<const int *>(sorted[at]), static_cast<const int *>(order[at]), (int)n,                \
-                           static_cast<const E *>(grad), grad_stride, vocab, dim, scale, static_cast<E *>(grad_weight),      \
-                           partial, pieces, shift);                                                                          \
-        if (pieces > 1)                                                                                                      \
-            hipLaunchKernelGGL((embed_join_kernel<DT, VEC>), dim3((unsigned)pieces), dim3(kBlock), 0, st,                    \
-                               static_cast<const int *>(sorted[at]), (int)n, vocab, dim, scale, static_cast<E *>(grad_weight), \
-                               static_cast<const float *>(partial), pieces);                                                 \
-    } while (0)
-    if (vec)
-        EMBED_SUM(DT::EPC);
-    else
-        EMBED_SUM(1);
-#undef EMBED_SUM
+    const int shift = row_shift(dim, VEC), piece = piece_of(n), pieces = pieces_of(n);
+    const int slices = (dim + (VEC << shift) - 1) / (VEC << shift);
+    const long long blocks = ((((long long)pieces * slices) << shift) + kBlock - 1) / kBlock;
+    const long long zero_blocks = n <= kRankMax ? 0 : ((vocab - 1) / 16 / (kBlock / kWave)) + 1;
+    if (blocks + zero_blocks > 0x7fffffffll) return RNNT_STATUS_INVALID_VALUE;
+    hipLaunchKernelGGL((embed_sum_kernel<DT, VEC>), dim3((unsigned)(blocks + zero_blocks)), dim3(kBlock), 0, st,
+                       static_cast<const int *>(sorted[at]), static_cast<const int *>(order[at]), n, grad, grad_stride, vocab, dim, scale,
+                       grad_weight, partial, piece, pieces, slices, shift, (unsigned)blocks);
+    if (pieces > 1)
+        hipLaunchKernelGGL((embed_join_kernel<DT, VEC>), dim3((unsigned)pieces, (unsigned)((dim + kWave * VEC - 1) / (kWave * VEC))),
+                           dim3(kJoinWaves * kWave), 0, st, static_cast<const int *>(sorted[at]), n, vocab, dim, scale, grad_weight,
+                           static_cast<const float *>(partial), piece);
     return hipGetLastError() == hipSuccess ? RNNT_STATUS_SUCCESS : RNNT_STATUS_EXECUTION_FAILED;
+}
+
+template <typename DT>
+rnntStatus_t embed_backward(const void *tokens, int tokens_64, long long n, const void *grad, long long grad_stride, int vocab,
+                            int dim, float scale, long long padding, void *grad_weight, void *workspace, hipStream_t st) {
+    typedef typename DT::elem E;
+    const bool vec = dim % DT::EPC == 0 && grad_stride % DT::EPC == 0 && aligned16(grad) && aligned16(grad_weight);
+    return (vec ? embed_backward_with<DT, DT::EPC> : embed_backward_with<DT, 1>)(tokens, tokens_64, (int)n, static_cast<const E *>(grad),
+                                                                               grad_stride, vocab, dim, scale, padding,
+                                                                               static_cast<E *>(grad_weight), workspace, st);
 }
 
 }  // namespace

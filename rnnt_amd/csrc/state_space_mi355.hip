@@ -200,7 +200,16 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
             if (!LOCAL && zp) zn[j] = zp[tt * a.z_time];
         }
     };
-    if (te > t0) fetch(t0);
+    // the next step's B and C are under way while a step is computed (32 states of both would not fit the scalar registers)
+    constexpr bool kNext = N <= 16;
+    ScalarRow<DT, N> Bn, Cn;
+    if (te > t0) {
+        fetch(t0);
+        if (kNext) {
+            Bn.load(Bp + t0 * a.B_time);
+            if (!LOCAL) Cn.load(Cp + t0 * a.C_time);
+        }
+    }
     for (int tb = t0; tb < te; tb += kAhead) {
         E xc[kAhead], dtc[kAhead], zc[kAhead];
 #pragma unroll
@@ -216,9 +225,14 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
         for (int j = 0; j < kAhead; ++j) {
             const int t = tb + j;
             if (t >= te) break;
-            ScalarRow<DT, N> B, C;
-            B.load(Bp + t * a.B_time);
-            if (!LOCAL) C.load(Cp + t * a.C_time);
+            ScalarRow<DT, N> B = Bn, C = Cn;
+            const long long ts = !kNext ? t : (t + 1 < te ? t + 1 : t);
+            Bn.load(Bp + ts * a.B_time);
+            if (!LOCAL) Cn.load(Cp + ts * a.C_time);
+            if (!kNext) {
+                B = Bn;
+                C = Cn;
+            }
             float sig;
             const float x = DT::to_float(xc[j]);
             const float delta = softplus_(DT::to_float(dtc[j]) + bias, sig);
@@ -678,7 +692,10 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const rnntScan a) {
 // ---------------------------------------------------------------------------------------------
 // causal convolution
 // ---------------------------------------------------------------------------------------------
-constexpr int kRun = 32;  // steps a thread walks
+// A wave takes 64 channels of a run of steps; the waves of a workgroup take neighbouring runs of the same channels.
+constexpr int kRunForward = 32, kRunBackward = 64;
+constexpr int kConvAhead = 8;  // steps loaded at once
+constexpr int kConvWaves = 4;
 
 // row t of xe - (W - 1) rows: x for t >= 0, the initial state (zeros) before
 template <typename DT, int W>
@@ -689,38 +706,49 @@ __device__ __forceinline__ float conv_in(const rnntConv &c, int b, long long t, 
 }
 
 template <typename DT, int W>
-__global__ __launch_bounds__(256) void conv_forward_kernel(const rnntConv c, int runs, int blocks_d) {
+__global__ __launch_bounds__(kConvWaves *kWave) void conv_forward_kernel(const rnntConv c, int runs, int groups) {
     typedef typename DT::elem E;
-    const int d = (int)(blockIdx.x % blocks_d) * 256 + threadIdx.x;
-    const int rest = blockIdx.x / blocks_d;
-    const int run = rest % runs, b = rest / runs;
-    if (d >= c.dim) return;
-    const int len = clamp_len(c.lengths, b, c.length);
-    const int t0 = run * kRun, t1 = t0 + kRun < c.length ? t0 + kRun : c.length;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int d = (int)(blockIdx.x % groups) * kWave + lane;
+    const long long item = (long long)(blockIdx.x / groups) * kConvWaves + wave;
+    const int run = (int)(item % runs);
+    const long long b = item / runs;
+    if (b >= c.batch || d >= c.dim) return;
+    const int len = clamp_len(c.lengths, (int)b, c.length);
+    const int t0 = run * kRunForward, t1 = t0 + kRunForward < c.length ? t0 + kRunForward : c.length;
     const int te = len < t1 ? (len > t0 ? len : t0) : t1;
     float w[W], win[W];
 #pragma unroll
     for (int k = 0; k < W; ++k) w[k] = c.weight[(size_t)d * W + k];
     const float bias = c.bias ? c.bias[d] : 0.f;
+    const E *x = static_cast<const E *>(c.x) + b * c.x_batch + d;
     E *y = static_cast<E *>(c.y) + (size_t)b * c.length * c.dim + d;
     if (te > t0) {
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) win[k + 1] = conv_in<DT, W>(c, b, (long long)t0 - (W - 1) + k, d);
+        for (int k = 0; k < W - 1; ++k) win[k + 1] = conv_in<DT, W>(c, (int)b, (long long)t0 - (W - 1) + k, d);
     }
-    for (int t = t0; t < te; ++t) {
+    for (int tb = t0; tb < te; tb += kConvAhead) {
+        E in[kConvAhead];
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) win[k] = win[k + 1];
-        win[W - 1] = conv_in<DT, W>(c, b, t, d);
-        float p = bias;
+        for (int j = 0; j < kConvAhead; ++j) in[j] = x[(long long)(tb + j < te ? tb + j : te - 1) * c.x_time];
 #pragma unroll
-        for (int k = 0; k < W; ++k) p = fma_(w[k], win[k], p);
-        y[(size_t)t * c.dim] = DT::from_float(c.silu ? p * sigmoid_(p) : p);
+        for (int j = 0; j < kConvAhead; ++j) {
+            if (tb + j >= te) break;
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) win[k] = win[k + 1];
+            win[W - 1] = DT::to_float(in[j]);
+            float p = bias;
+#pragma unroll
+            for (int k = 0; k < W; ++k) p = fma_(w[k], win[k], p);
+            y[(size_t)(tb + j) * c.dim] = DT::from_float(c.silu ? p * sigmoid_(p) : p);
+        }
     }
     for (int t = te; t < t1; ++t) y[(size_t)t * c.dim] = DT::from_float(0.f);
     if (run == 0 && c.final_state) {
         float fin[W - 1];  // (all read before any is written: final_state may be the buffer of initial_state)
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) fin[k] = conv_in<DT, W>(c, b, (long long)len - (W - 1) + k, d);
+        for (int k = 0; k < W - 1; ++k) fin[k] = conv_in<DT, W>(c, (int)b, (long long)len - (W - 1) + k, d);
         E *f = static_cast<E *>(c.final_state) + (size_t)b * (W - 1) * c.dim + d;
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) f[(size_t)k * c.dim] = DT::from_float(fin[k]);
@@ -728,84 +756,141 @@ __global__ __launch_bounds__(256) void conv_forward_kernel(const rnntConv c, int
 }
 
 // dxe[e] = sum_k w[k] gp[e - k] + grad_final, dw[k] = sum_t gp[t] xe[t + k], db = sum gp, with gp = grad_y silu'(p):
-// p is formed again from the W rows that the window holds.  partial: [batch * runs][W + 1][dim].
+// p is formed again from the W rows that the window holds.  partial: [workgroups of one channel group][W + 1][dim].
 template <typename DT, int W>
-__global__ __launch_bounds__(256) void conv_backward_kernel(const rnntConv c, int runs, int blocks_d, float *partial) {
+__global__ __launch_bounds__(kConvWaves *kWave) void conv_backward_kernel(const rnntConv c, int runs, int groups, float *partial) {
     typedef typename DT::elem E;
-    const int d = (int)(blockIdx.x % blocks_d) * 256 + threadIdx.x;
-    const int rest = blockIdx.x / blocks_d;
-    const int run = rest % runs, b = rest / runs;
-    if (d >= c.dim) return;
-    const int len = clamp_len(c.lengths, b, c.length);
-    const int t0 = run * kRun, t1 = t0 + kRun < c.length ? t0 + kRun : c.length;
-    float w[W], win[W], gp[W], dw[W], db = 0.f;
+    __shared__ float s_sum[kConvWaves][W + 1][kWave];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int d0 = (int)(blockIdx.x % groups) * kWave + lane;
+    const bool ok = d0 < c.dim;
+    const int d = ok ? d0 : c.dim - 1;
+    const long long item = (long long)(blockIdx.x / groups) * kConvWaves + wave;
+    const int run = (int)(item % runs);
+    const long long b = item / runs;
+    float dw[W], db = 0.f;
 #pragma unroll
-    for (int k = 0; k < W; ++k) {
-        w[k] = c.weight[(size_t)d * W + k];
-        dw[k] = 0.f;
-        gp[k] = 0.f;
-        win[k] = 0.f;
-    }
-    const float bias = c.bias ? c.bias[d] : 0.f;
-    const E *gy = static_cast<const E *>(c.grad_y) + b * c.grad_y_batch + d;
-    E *dx = static_cast<E *>(c.grad_x) + (size_t)b * c.length * c.dim + d;
-    E *di = c.grad_initial ? static_cast<E *>(c.grad_initial) + (size_t)b * (W - 1) * c.dim + d : nullptr;
-    const E *gf = c.grad_final ? static_cast<const E *>(c.grad_final) + (size_t)b * (W - 1) * c.dim + d : nullptr;
-    // rows of dxe that this run writes: its own steps' x rows t0 .. t1-1 and, run 0, the W - 1 rows of the initial state
-    const int first = run == 0 ? -(W - 1) : t0;
-    if (first < len) {
+    for (int k = 0; k < W; ++k) dw[k] = 0.f;
+    if (b < c.batch) {
+        const int len = clamp_len(c.lengths, (int)b, c.length);
+        const int t0 = run * kRunBackward, t1 = t0 + kRunBackward < c.length ? t0 + kRunBackward : c.length;
+        float w[W], win[W], gp[W];
 #pragma unroll
-        for (int k = 0; k < W - 1; ++k) win[k + 1] = first - (W - 1) + k >= -(W - 1) ? conv_in<DT, W>(c, b, (long long)first - (W - 1) + k, d) : 0.f;
-    }
-    // gp index: gp[k] = gp at step s - (W - 1) + k, where s is the newest step formed
-    for (int s = first; s < t1 + W - 1; ++s) {
-#pragma unroll
-        for (int k = 0; k < W - 1; ++k) {
-            win[k] = win[k + 1];
-            gp[k] = gp[k + 1];
+        for (int k = 0; k < W; ++k) {
+            w[k] = c.weight[(size_t)d * W + k];
+            gp[k] = 0.f;
+            win[k] = 0.f;
         }
-        gp[W - 1] = 0.f;
-        win[W - 1] = s < len ? conv_in<DT, W>(c, b, s, d) : 0.f;
-        if (s >= 0 && s < len) {
+        const float bias = c.bias ? c.bias[d] : 0.f;
+        const E *x = static_cast<const E *>(c.x) + b * c.x_batch + d;
+        const E *gy = static_cast<const E *>(c.grad_y) + b * c.grad_y_batch + d;
+        E *dx = static_cast<E *>(c.grad_x) + (size_t)b * c.length * c.dim + d;
+        E *di = c.grad_initial ? static_cast<E *>(c.grad_initial) + (size_t)b * (W - 1) * c.dim + d : nullptr;
+        const E *gf = c.grad_final ? static_cast<const E *>(c.grad_final) + (size_t)b * (W - 1) * c.dim + d : nullptr;
+        // Step s is newest in the window, gp[k] belongs to step s - (W - 1) + k; row t = s - (W - 1) of dx is then complete.
+        auto step = [&](int s, float xs, float gs, bool own) {
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) {
+                win[k] = win[k + 1];
+                gp[k] = gp[k + 1];
+            }
+            win[W - 1] = xs;
             float p = bias;
 #pragma unroll
             for (int k = 0; k < W; ++k) p = fma_(w[k], win[k], p);
-            float v = DT::to_float(gy[s * c.grad_y_time]);
+            float v = gs;
             if (c.silu) {
                 const float sg = sigmoid_(p);
                 v *= fma_(p * sg, 1.f - sg, sg);
             }
             gp[W - 1] = v;
-            if (s < t1) {  // (steps past t1 belong to the next run)
+            if (own) {  // (steps past t1 belong to the next run)
                 db += v;
 #pragma unroll
                 for (int k = 0; k < W; ++k) dw[k] = fma_(v, win[k], dw[k]);
             }
-        }
-        const int t = s - (W - 1);  // row whose W steps t .. s are now in gp[0 .. W-1]
-        if (t < first) continue;
-        float v = 0.f;
+        };
+        auto gradient = [&]() {
+            float v = 0.f;
 #pragma unroll
-        for (int k = 0; k < W; ++k) v = fma_(w[W - 1 - k], gp[k], v);
-        if (gf && t >= len - (W - 1) && t < len) v += DT::to_float(gf[(size_t)(t - (len - (W - 1))) * c.dim]);
-        if (t >= 0) {
-            dx[(size_t)t * c.dim] = DT::from_float(t < len ? v : 0.f);
-        } else if (di) {
-            di[(size_t)(t + W - 1) * c.dim] = DT::from_float(v);
+            for (int k = 0; k < W; ++k) v = fma_(w[W - 1 - k], gp[k], v);
+            return v;
+        };
+        auto finish = [&](int t) {  // row t of dx, or of the initial state's gradient; any t
+            float v = gradient();
+            if (gf && t >= len - (W - 1) && t < len) v += DT::to_float(gf[(size_t)(t - (len - (W - 1))) * c.dim]);
+            if (!ok) return;
+            if (t >= 0)
+                dx[(size_t)t * c.dim] = DT::from_float(t < len ? v : 0.f);
+            else if (di)
+                di[(size_t)(t + W - 1) * c.dim] = DT::from_float(v);
+        };
+        // rows of dxe that this run writes: its own steps' x rows t0 .. t1-1 and, run 0, the W - 1 rows of the initial state
+        const int first = run == 0 ? -(W - 1) : t0;
+        if (first < len) {
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k)
+                win[k + 1] = first - (W - 1) + k >= -(W - 1) ? conv_in<DT, W>(c, (int)b, (long long)first - (W - 1) + k, d) : 0.f;
+        }
+        int s = first;
+        const int stop = t1 + W - 1;
+        while (s < stop) {
+            // whole blocks inside the sequence and the run, whose dx rows are ordinary ones: loads first, no tests
+            if (s >= W - 1 && s - (W - 1) >= first && s + kConvAhead <= t1 && s + kConvAhead <= len - (W - 1)) {
+                E xin[kConvAhead], gin[kConvAhead];
+#pragma unroll
+                for (int j = 0; j < kConvAhead; ++j) {
+                    xin[j] = x[(long long)(s + j) * c.x_time];
+                    gin[j] = gy[(long long)(s + j) * c.grad_y_time];
+                }
+#pragma unroll
+                for (int j = 0; j < kConvAhead; ++j) {
+                    step(s + j, DT::to_float(xin[j]), DT::to_float(gin[j]), true);
+                    const float v = gradient();
+                    if (ok) dx[(size_t)(s + j - (W - 1)) * c.dim] = DT::from_float(v);
+                }
+                s += kConvAhead;
+                continue;
+            }
+            const bool live = s >= 0 && s < len;
+            step(s, s < len ? conv_in<DT, W>(c, (int)b, s, d) : 0.f, live ? DT::to_float(gy[(long long)s * c.grad_y_time]) : 0.f,
+                 live && s < t1);
+            if (!live) gp[W - 1] = 0.f;  // (0 times an infinite derivative)
+            if (s - (W - 1) >= first) finish(s - (W - 1));
+            ++s;
         }
     }
-    float *o = partial + (size_t)(b * runs + run) * (W + 1) * c.dim + d;
 #pragma unroll
-    for (int k = 0; k < W; ++k) o[(size_t)k * c.dim] = dw[k];
-    o[(size_t)W * c.dim] = db;
+    for (int k = 0; k < W; ++k) s_sum[wave][k][lane] = dw[k];
+    s_sum[wave][W][lane] = db;
+    __syncthreads();
+    for (int k = wave; k <= W; k += kConvWaves) {
+        float v = 0.f;
+#pragma unroll
+        for (int q = 0; q < kConvWaves; ++q) v += s_sum[q][k][lane];
+        if (ok) partial[((size_t)(blockIdx.x / groups) * (W + 1) + k) * c.dim + d] = v;
+    }
 }
 
+// 64 columns of the partial sums per workgroup, its 16 waves a range of the parts each
 template <int W>
-__global__ __launch_bounds__(256) void conv_backward_sum_kernel(const rnntConv c, const float *partial, int parts) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i >= (W + 1) * c.dim) return;
+__global__ __launch_bounds__(1024) void conv_backward_sum_kernel(const rnntConv c, const float *partial, int parts) {
+    __shared__ float s_sum[16][kWave];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const int i = blockIdx.x * kWave + lane, columns = (W + 1) * c.dim;
+    const int per = (parts + 15) / 16, p0 = wave * per, p1 = p0 + per < parts ? p0 + per : parts;
     float s = 0.f;
-    for (int p = 0; p < parts; ++p) s += partial[(size_t)p * (W + 1) * c.dim + i];
+    if (i < columns) {
+#pragma unroll 8
+        for (int p = p0; p < p1; ++p) s += partial[(size_t)p * columns + i];
+    }
+    s_sum[wave][lane] = s;
+    __syncthreads();
+    if (wave != 0 || i >= columns) return;
+    s = 0.f;
+#pragma unroll
+    for (int q = 0; q < 16; ++q) s += s_sum[q][lane];
     const int k = i / c.dim, d = i - k * c.dim;
     if (k < W)
         c.grad_weight[(size_t)d * W + k] = s;
@@ -958,29 +1043,32 @@ rnntStatus_t scan_step(const rnntScan &a, hipStream_t st) {
         }                                                                      \
     } while (0)
 
-inline int runs_of(int length) { return (length + kRun - 1) / kRun; }
+inline int runs_of(int length, int run) { return (length + run - 1) / run; }
+inline long long conv_items(int batch, int length, int run) {  // workgroups per channel group
+    return ((long long)batch * runs_of(length, run) + kConvWaves - 1) / kConvWaves;
+}
 
 inline bool conv_shape_ok(int batch, int length, int dim, int width) {
     return batch >= 1 && length >= 1 && dim >= 1 && width >= 2 && width <= 4 && length <= (1 << 30) &&
            (long long)batch * length < (1ll << 31) && (long long)batch * dim < (1ll << 31) &&
-           (long long)dim * 8 < (1ll << 31) && (long long)batch * runs_of(length) * ((dim + 255) / 256) < (1ll << 31);
+           (long long)dim * 8 < (1ll << 31) && conv_items(batch, length, kRunForward) * groups_of(dim) < (1ll << 31);
 }
 
 template <typename DT, int W>
 rnntStatus_t conv_forward(const rnntConv &c, hipStream_t st) {
-    const int runs = runs_of(c.length), blocks = (c.dim + 255) / 256;
-    hipLaunchKernelGGL((conv_forward_kernel<DT, W>), dim3((unsigned)((long long)c.batch * runs * blocks)), dim3(256), 0, st, c,
-                       runs, blocks);
+    const unsigned grid = (unsigned)(conv_items(c.batch, c.length, kRunForward) * groups_of(c.dim));
+    hipLaunchKernelGGL((conv_forward_kernel<DT, W>), dim3(grid), dim3(kConvWaves * kWave), 0, st, c, runs_of(c.length, kRunForward),
+                       groups_of(c.dim));
     return launched();
 }
 template <typename DT, int W>
 rnntStatus_t conv_backward(const rnntConv &c, hipStream_t st) {
-    const int runs = runs_of(c.length), blocks = (c.dim + 255) / 256;
+    const int parts = (int)conv_items(c.batch, c.length, kRunBackward);
     float *partial = static_cast<float *>(c.workspace);
-    hipLaunchKernelGGL((conv_backward_kernel<DT, W>), dim3((unsigned)((long long)c.batch * runs * blocks)), dim3(256), 0, st, c,
-                       runs, blocks, partial);
-    hipLaunchKernelGGL((conv_backward_sum_kernel<W>), dim3((unsigned)(((W + 1) * c.dim + 255) / 256)), dim3(256), 0, st, c,
-                       static_cast<const float *>(partial), c.batch * runs);
+    hipLaunchKernelGGL((conv_backward_kernel<DT, W>), dim3((unsigned)((long long)parts * groups_of(c.dim))), dim3(kConvWaves * kWave), 0,
+                       st, c, runs_of(c.length, kRunBackward), groups_of(c.dim), partial);
+    hipLaunchKernelGGL((conv_backward_sum_kernel<W>), dim3((unsigned)(((long long)(W + 1) * c.dim + kWave - 1) / kWave)), dim3(1024), 0,
+                       st, c, static_cast<const float *>(partial), parts);
     return launched();
 }
 template <typename DT, int W>
@@ -1048,7 +1136,7 @@ rnntStatus_t rnnt_selective_scan_step(const rnntScan *scan) {
 
 rnntStatus_t rnnt_causal_conv_workspace_size(int batch, int length, int dim, int width, size_t *size_bytes) {
     if (size_bytes == nullptr || !conv_shape_ok(batch, length, dim, width)) return RNNT_STATUS_INVALID_VALUE;
-    *size_bytes = (size_t)batch * runs_of(length) * (width + 1) * dim * sizeof(float);
+    *size_bytes = (size_t)conv_items(batch, length, kRunBackward) * (width + 1) * dim * sizeof(float);
     return RNNT_STATUS_SUCCESS;
 }
 
