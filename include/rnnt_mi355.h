@@ -478,11 +478,11 @@ rnntStatus_t rnnt_causal_conv_step(const rnntConv *conv);
  * last dimension adjacent); A [dim, state], D, dt_bias [dim] fp32; initial_state, final_state [batch, dim, state]
  * fp32 contiguous; y contiguous.  state is 8, 16 or 32.  D, z, dt_bias, initial_state, final_state, lengths may be NULL
  * (lengths as above; a length of 0 gives back the initial state).
- * forward: chunk_states (NULL in inference) receives the state before every 16th step, rnnt_selective_scan_states_size
- * bytes, which backward reads.  backward: grad_y [batch, length, dim] (strides), grad_final NULL or contiguous;
+ * forward: chunk_states (NULL in inference) receives the state before every 16th step and B and C in fp32,
+ * rnnt_selective_scan_states_size bytes, 16-byte aligned, which backward reads.  backward: grad_y [batch, length, dim] (strides), grad_final NULL or contiguous;
  * grad_x, grad_dt, grad_z (NULL iff z is NULL) and grad_B, grad_C contiguous in the inputs' type, zero from lengths[b] on;
  * grad_A, grad_D, grad_dt_bias fp32 (the latter two may be NULL), grad_initial may be NULL.
- * workspace: rnnt_selective_scan_workspace_size bytes (0: may be NULL), 16-byte aligned, for forward and backward alike.
+ * workspace: rnnt_selective_scan_workspace_size bytes, 16-byte aligned, for forward (backward = 0) and backward (1).
  * step: one token per sequence (length is ignored, times strides too); reads initial_state (required), writes final_state
  * (required; may be the same buffer).
  */

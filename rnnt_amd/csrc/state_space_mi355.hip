@@ -20,6 +20,8 @@ namespace {
 
 using namespace rnnt_mi355_detail;
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 constexpr float kLog2e = 1.4426950408889634f, kLog2eLow = 1.925963033500e-08f, kLn2 = 0.6931471805599453f;
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -55,46 +57,26 @@ __device__ __forceinline__ float softplus_(float v, float &sig) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// B_t and C_t: N adjacent values at an address that is the same for the whole wave.  They are read through the scalar
-// cache into scalar registers, so that the recurrence's multiply-adds take them as scalar operands: no vector load, no
-// LDS, no register per lane.  Scalar loads are whole 4-byte words: a row of 16-bit values that starts in the middle of
-// a word is read from that word on and moved down by 16 bits.
+// B_t and C_t are the same for all channels of a sequence, so for a whole wave: the scan kernels read them through the
+// scalar cache into scalar registers, and the recurrence's multiply-adds take them as scalar operands: no vector load,
+// no LDS, no register per lane.  Scalar loads are whole aligned words, the scalar unit has no half-precision conversion,
+// and unpacking bf16 there costs as many issue slots as the recurrence itself (16 states: 100 scalar beside 105 vector
+// instructions a step, 0.73 us a step).  So a first small kernel lays both out as fp32, four states of B beside the
+// same four of C: a row is whole 32-byte loads for any wave, whatever type, stride or alignment the caller's have.
+// Rows from a sequence's length on, up to a multiple of 16 (and one row more at the end), are zero.
 // ---------------------------------------------------------------------------------------------
-typedef const __attribute__((address_space(4))) unsigned *scalar_words;
+typedef const __attribute__((address_space(4))) float *scalar_floats;
 
-template <typename DT, int N>
-struct ScalarRow {
-    static constexpr bool kHalf = sizeof(typename DT::elem) == 2;
-    static constexpr int kWords = kHalf ? N / 2 : N;
-    unsigned w[kWords];
-    __device__ __forceinline__ void load(const typename DT::elem *p) {
-        const unsigned long long at = reinterpret_cast<unsigned long long>(p);
-        scalar_words q = (scalar_words)(at & ~3ull);
-        if (!kHalf || (at & 2) == 0) {
+template <int N>
+struct ScalarRow {  // N states of B and of C
+    float v[2 * N];
+    __device__ __forceinline__ void load(const float *p) {
+        scalar_floats q = (scalar_floats) reinterpret_cast<unsigned long long>(p);
 #pragma unroll
-            for (int i = 0; i < kWords; ++i) w[i] = q[i];
-        } else {
-            unsigned prev = q[0];
-#pragma unroll
-            for (int i = 0; i < kWords; ++i) {
-                const unsigned next = q[i + 1];
-                w[i] = (unsigned)(((unsigned long long)next << 32 | prev) >> 16);
-                prev = next;
-            }
-        }
+        for (int i = 0; i < 2 * N; ++i) v[i] = q[i];
     }
-    __device__ __forceinline__ float operator[](int n) const {
-        if constexpr (!kHalf) {
-            return __uint_as_float(w[n]);
-        } else {
-            const unsigned v = w[n / 2];
-            if constexpr (sizeof(DT) && __is_same(DT, BF16)) {
-                return __uint_as_float(n & 1 ? v & 0xffff0000u : v << 16);
-            } else {
-                return (float)__builtin_bit_cast(_Float16, (unsigned short)(n & 1 ? v >> 16 : v & 0xffffu));
-            }
-        }
-    }
+    __device__ __forceinline__ float B(int n) const { return v[n / 4 * 8 + n % 4]; }
+    __device__ __forceinline__ float C(int n) const { return v[n / 4 * 8 + 4 + n % 4]; }
 };
 
 // ---------------------------------------------------------------------------------------------
@@ -112,12 +94,32 @@ struct ScanGeom {
     int seg_len;   // steps per segment, a multiple of kChunk
     float *seg_state;  // [batch][segments][state / 4][dim][4]: a segment's end from zero, then the state it starts from
     float *seg_delta;  // [batch][segments][dim]: sum of delta over the segment
+    float *rows;       // B and C: [batch][length rounded up to kChunk][2 state], and one row more
+    int padded;        // length rounded up to kChunk
 };
 
 __device__ __forceinline__ int clamp_len(const int *lengths, int b, int length) {
     if (lengths == nullptr) return length;
     const int n = lengths[b];
     return n < 0 ? 0 : (n > length ? length : n);
+}
+
+template <typename DT, int N>
+__global__ __launch_bounds__(256) void scan_rows_kernel(const rnntScan a, const ScanGeom g) {
+    typedef typename DT::elem E;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const int k = (int)(i % (2 * N));
+    const long long row = i / (2 * N);
+    const long long b = row / g.padded;
+    if (row > (long long)a.batch * g.padded) return;
+    const int t = (int)(row - b * g.padded);
+    float v = 0.f;
+    if (b < a.batch && t < clamp_len(a.lengths, (int)b, a.length)) {
+        const int n = k / 8 * 4 + k % 4;
+        v = DT::to_float(k % 8 < 4 ? static_cast<const E *>(a.B)[b * a.B_batch + t * a.B_time + n]
+                                   : static_cast<const E *>(a.C)[b * a.C_batch + t * a.C_time + n]);
+    }
+    g.rows[i] = v;
 }
 
 template <int N>
@@ -183,9 +185,10 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
     const float skip = !LOCAL && a.D ? a.D[d] : 0.f;
     const E *xp = static_cast<const E *>(a.x) + b * a.x_batch + d;
     const E *dtp = static_cast<const E *>(a.dt) + b * a.dt_batch + d;
-    const E *zp = a.z && !LOCAL ? static_cast<const E *>(a.z) + b * a.z_batch + d : nullptr;
-    const E *Bp = static_cast<const E *>(a.B) + b * a.B_batch;
-    const E *Cp = static_cast<const E *>(a.C) + b * a.C_batch;
+    const bool gated = a.z != nullptr;  // (without a gate its loads repeat x's: no branch between loads)
+    const E *zp = gated ? static_cast<const E *>(a.z) + b * a.z_batch + d : xp;
+    const long long z_time = gated ? a.z_time : a.x_time;
+    const float *rows = g.rows + ((size_t)b * g.padded + t0) * 2 * N;
     E *yp = LOCAL ? nullptr : static_cast<E *>(a.y) + (size_t)b * a.length * a.dim + d;
     const int chunks = (a.length + kChunk - 1) / kChunk;
     float sum_delta = 0.f;
@@ -197,18 +200,15 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
             const long long tt = t + j < te ? t + j : te - 1;
             xn[j] = xp[tt * a.x_time];
             dtn[j] = dtp[tt * a.dt_time];
-            if (!LOCAL && zp) zn[j] = zp[tt * a.z_time];
+            if (!LOCAL) zn[j] = zp[tt * z_time];
         }
     };
-    // the next step's B and C are under way while a step is computed (32 states of both would not fit the scalar registers)
+    // the next step's row is under way while a step is computed (32 states of two rows would not fit the scalar registers)
     constexpr bool kNext = N <= 16;
-    ScalarRow<DT, N> Bn, Cn;
+    ScalarRow<N> next;
     if (te > t0) {
         fetch(t0);
-        if (kNext) {
-            Bn.load(Bp + t0 * a.B_time);
-            if (!LOCAL) Cn.load(Cp + t0 * a.C_time);
-        }
+        if (kNext) next.load(rows);
     }
     for (int tb = t0; tb < te; tb += kAhead) {
         E xc[kAhead], dtc[kAhead], zc[kAhead];
@@ -225,14 +225,10 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
         for (int j = 0; j < kAhead; ++j) {
             const int t = tb + j;
             if (t >= te) break;
-            ScalarRow<DT, N> B = Bn, C = Cn;
-            const long long ts = !kNext ? t : (t + 1 < te ? t + 1 : t);
-            Bn.load(Bp + ts * a.B_time);
-            if (!LOCAL) Cn.load(Cp + ts * a.C_time);
-            if (!kNext) {
-                B = Bn;
-                C = Cn;
-            }
+            ScalarRow<N> row = next;
+            if (!kNext) row.load(rows);
+            rows += 2 * N;
+            if (kNext) next.load(rows);
             float sig;
             const float x = DT::to_float(xc[j]);
             const float delta = softplus_(DT::to_float(dtc[j]) + bias, sig);
@@ -240,18 +236,18 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
             float y0 = 0.f, y1 = 0.f;  // (two chains)
 #pragma unroll
             for (int n = 0; n < N; n += 2) {
-                h[n] = fma_(exp2_(delta * A2[n]), h[n], dx * B[n]);
-                h[n + 1] = fma_(exp2_(delta * A2[n + 1]), h[n + 1], dx * B[n + 1]);
+                h[n] = fma_(exp2_(delta * A2[n]), h[n], dx * row.B(n));
+                h[n + 1] = fma_(exp2_(delta * A2[n + 1]), h[n + 1], dx * row.B(n + 1));
                 if (!LOCAL) {
-                    y0 = fma_(C[n], h[n], y0);
-                    y1 = fma_(C[n + 1], h[n + 1], y1);
+                    y0 = fma_(row.C(n), h[n], y0);
+                    y1 = fma_(row.C(n + 1), h[n + 1], y1);
                 }
             }
             if (LOCAL) {
                 sum_delta += delta;
             } else {
                 float y = fma_(skip, x, y0 + y1);
-                if (zp) {
+                if (gated) {
                     const float z = DT::to_float(zc[j]);
                     y *= z * sigmoid_(z);
                 }
@@ -332,9 +328,11 @@ __global__ __launch_bounds__(64) void scan_backward_local_kernel(const rnntScan 
     for (int n = 0; n < N; ++n) G[n] = 0.f;
     const float bias = a.dt_bias ? a.dt_bias[d] : 0.f;
     const E *dtp = static_cast<const E *>(a.dt) + b * a.dt_batch + d;
-    const E *zp = a.z ? static_cast<const E *>(a.z) + b * a.z_batch + d : nullptr;
+    const bool gated = a.z != nullptr;
+    const E *zp = gated ? static_cast<const E *>(a.z) + b * a.z_batch + d : dtp;
+    const long long z_time = gated ? a.z_time : a.dt_time;
     const E *gp = static_cast<const E *>(a.grad_y) + b * a.grad_y_batch + d;
-    const E *Cp = static_cast<const E *>(a.C) + b * a.C_batch;
+    const float *rows = g.rows + ((size_t)b * g.padded + te) * 2 * N;  // one past the step
     float sum_delta = 0.f;
     E dtn[kAhead], zn[kAhead], gn[kAhead];
     auto fetch = [&](int t) {  // steps t, t - 1, ...
@@ -343,7 +341,7 @@ __global__ __launch_bounds__(64) void scan_backward_local_kernel(const rnntScan 
             const long long tt = t - j > t0 ? t - j : t0;
             dtn[j] = dtp[tt * a.dt_time];
             gn[j] = gp[tt * a.grad_y_time];
-            if (zp) zn[j] = zp[tt * a.z_time];
+            zn[j] = zp[tt * z_time];
         }
     };
     if (te > t0) fetch(te - 1);
@@ -360,18 +358,19 @@ __global__ __launch_bounds__(64) void scan_backward_local_kernel(const rnntScan 
         for (int j = 0; j < kAhead; ++j) {
             const int t = tb - j;
             if (t < t0) break;
-            ScalarRow<DT, N> C;
-            C.load(Cp + t * a.C_time);
+            rows -= 2 * N;
+            ScalarRow<N> row;
+            row.load(rows);
             float sig;
             const float delta = softplus_(DT::to_float(dtc[j]) + bias, sig);
             float gy = DT::to_float(gc[j]);
-            if (zp) {
+            if (gated) {
                 const float z = DT::to_float(zc[j]);
                 gy *= z * sigmoid_(z);
             }
             sum_delta += delta;
 #pragma unroll
-            for (int n = 0; n < N; ++n) G[n] = exp2_(delta * A2[n]) * fma_(C[n], gy, G[n]);
+            for (int n = 0; n < N; ++n) G[n] = exp2_(delta * A2[n]) * fma_(row.C(n), gy, G[n]);
         }
     }
     if (ok) {
@@ -475,13 +474,14 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
     const float skip = a.D ? a.D[d] : 0.f;
     const E *xp = static_cast<const E *>(a.x) + b * a.x_batch + d;
     const E *dtp = static_cast<const E *>(a.dt) + b * a.dt_batch + d;
-    const E *zp = a.z ? static_cast<const E *>(a.z) + b * a.z_batch + d : nullptr;
+    const bool gated = a.z != nullptr;
+    const E *zp = gated ? static_cast<const E *>(a.z) + b * a.z_batch + d : xp;
+    const long long z_time = gated ? a.z_time : a.x_time;
     const E *gp = static_cast<const E *>(a.grad_y) + b * a.grad_y_batch + d;
-    const E *Bp = static_cast<const E *>(a.B) + b * a.B_batch + wave * S;
-    const E *Cp = static_cast<const E *>(a.C) + b * a.C_batch + wave * S;
+    const float *rows = g.rows + (size_t)b * g.padded * 2 * N + wave * 2 * S;
     const size_t out0 = (size_t)b * a.length * a.dim + d;
     E *dxp = static_cast<E *>(a.grad_x) + out0, *ddtp = static_cast<E *>(a.grad_dt) + out0;
-    E *dzp = a.z ? static_cast<E *>(a.grad_z) + out0 : nullptr;
+    E *dzp = gated ? static_cast<E *>(a.grad_z) + out0 : nullptr;
     float dD = 0.f, dbias = 0.f;
 
     if (ok) {
@@ -491,19 +491,35 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
             if (dzp) dzp[(size_t)t * a.dim] = DT::from_float(0.f);
         }
     }
-    for (int c = (te - 1) / kChunk; te > t0 && c >= t0 / kChunk; --c) {
+    // a chunk's inputs are under way while the chunk after it is computed
+    E xn[kMine], dtn[kMine], zn[kMine], gn[kMine];
+    f32x4 hn;
+    auto fetch = [&](int c) {
+#pragma unroll
+        for (int j = 0; j < kMine; ++j) {
+            const int t = c * kChunk + wave * kMine + j;
+            const long long tt = t < te ? t : te - 1;
+            xn[j] = xp[tt * a.x_time];
+            dtn[j] = dtp[tt * a.dt_time];
+            zn[j] = zp[tt * z_time];
+            gn[j] = gp[tt * a.grad_y_time];
+        }
+        hn = *reinterpret_cast<const f32x4 *>(a.chunk_states + ((size_t)b * chunks + c) * N * a.dim + ((size_t)wave * a.dim + d) * 4);
+    };
+    const int c0 = t0 / kChunk;
+    if (te > t0) fetch((te - 1) / kChunk);
+    for (int c = (te - 1) / kChunk; te > t0 && c >= c0; --c) {
         const int tc = c * kChunk;
         float sigv[kMine], dzf[kMine];
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
             const int i = wave * kMine + j, t = tc + i;
-            const long long tt = t < te ? t : te - 1;
-            const float x = DT::to_float(xp[tt * a.x_time]);
-            float delta = softplus_(DT::to_float(dtp[tt * a.dt_time]) + bias, sigv[j]);
-            float gy = DT::to_float(gp[tt * a.grad_y_time]);
+            const float x = DT::to_float(xn[j]);
+            const float delta = softplus_(DT::to_float(dtn[j]) + bias, sigv[j]);
+            float gy = DT::to_float(gn[j]);
             dzf[j] = 0.f;
-            if (zp) {
-                const float z = DT::to_float(zp[tt * a.z_time]), s = sigmoid_(z);
+            if (gated) {
+                const float z = DT::to_float(zn[j]), s = sigmoid_(z);
                 dzf[j] = gy * fma_(z * s, 1.f - s, s);
                 gy *= z * s;
             }
@@ -512,45 +528,39 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
             s_x[i][lane] = in ? x : 0.f;
             s_gy[i][lane] = in ? gy : 0.f;
         }
-        float h[S];
-        const float *tile = a.chunk_states + ((size_t)b * chunks + c) * N * a.dim;
-#pragma unroll
-        for (int n = 0; n < S; ++n) h[n] = *tile_at(tile, wave * S + n);
+        float h[S] = {hn.x, hn.y, hn.z, hn.w};
+        if (c > c0) fetch(c - 1);
         __syncthreads();
 
         float before[kChunk][S], decay[kChunk][S];
 #pragma unroll
         for (int i = 0; i < kChunk; ++i) {
-            const long long tt = tc + i < te ? tc + i : te - 1;
-            ScalarRow<DT, S> B, C;
-            B.load(Bp + tt * a.B_time);
-            C.load(Cp + tt * a.C_time);
+            ScalarRow<S> row;
+            row.load(rows + (size_t)(tc + i) * 2 * N);
             const float delta = s_delta[i][lane], dx = delta * s_x[i][lane];
             float y = 0.f;
 #pragma unroll
             for (int n = 0; n < S; ++n) {
                 before[i][n] = h[n];
                 decay[i][n] = exp2_(delta * A2[n]);
-                h[n] = fma_(decay[i][n], h[n], dx * B[n]);
-                y = fma_(C[n], h[n], y);
+                h[n] = fma_(decay[i][n], h[n], dx * row.B(n));
+                y = fma_(row.C(n), h[n], y);
             }
             s_part[0][wave][i][lane] = y;
         }
 #pragma unroll
         for (int i = kChunk - 1; i >= 0; --i) {
-            const long long tt = tc + i < te ? tc + i : te - 1;
-            ScalarRow<DT, S> B, C;
-            B.load(Bp + tt * a.B_time);
-            C.load(Cp + tt * a.C_time);
+            ScalarRow<S> row;
+            row.load(rows + (size_t)(tc + i) * 2 * N);
             const float delta = s_delta[i][lane], dx = delta * s_x[i][lane], gy = s_gy[i][lane];
             float inner = 0.f, rate = 0.f, sums[2 * S];
 #pragma unroll
             for (int n = 0; n < S; ++n) {
                 const float after = i + 1 < kChunk ? before[i + 1 < kChunk ? i + 1 : 0][n] : h[n];
-                const float gn = fma_(C[n], gy, G[n]);
+                const float gn = fma_(row.C(n), gy, G[n]);
                 sums[n] = gn * dx;
                 sums[S + n] = after * gy;
-                inner = fma_(gn, B[n], inner);
+                inner = fma_(gn, row.B(n), inner);
                 G[n] = gn * decay[i][n];
                 const float r = G[n] * before[i][n];
                 dA[n] = fma_(r, delta, dA[n]);
@@ -615,13 +625,14 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
 }
 
 // dB, dC: the channel groups' shares of every step, in order; dA, dD, ddt_bias: the shares of sequences and segments.
-// Blocks [0, bc_blocks) take the steps, the others the parameters (256 sums each).
+// Workgroups [0, bc_blocks) take 1024 values of the steps each, the others 64 columns of the parameters, their 16 waves a
+// range of the shares each.
 template <typename DT, int N>
-__global__ __launch_bounds__(256) void scan_backward_sum_kernel(const rnntScan a, const ScanGeom g, const ScanPartials in,
-                                                                unsigned bc_blocks) {
+__global__ __launch_bounds__(1024) void scan_backward_sum_kernel(const rnntScan a, const ScanGeom g, const ScanPartials in,
+                                                                 unsigned bc_blocks) {
     typedef typename DT::elem E;
     if (blockIdx.x < bc_blocks) {
-        const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+        const long long i = (long long)blockIdx.x * 1024 + threadIdx.x;
         const int k = (int)(i % (2 * N));
         const long long row = i / (2 * N);
         if (row >= (long long)a.batch * a.length) return;
@@ -629,23 +640,36 @@ __global__ __launch_bounds__(256) void scan_backward_sum_kernel(const rnntScan a
         float s = 0.f;
         if (t < clamp_len(a.lengths, b, a.length)) {
             const float *p = in.BC + (size_t)row * g.groups * 2 * N + k;
+#pragma unroll 8
             for (int j = 0; j < g.groups; ++j) s += p[(size_t)j * 2 * N];
         }
         E *o = static_cast<E *>(k < N ? a.grad_B : a.grad_C);
         o[(size_t)row * N + (k < N ? k : k - N)] = DT::from_float(s);
         return;
     }
-    const long long i = (long long)(blockIdx.x - bc_blocks) * 256 + threadIdx.x;
-    const int parts = a.batch * g.segments;
-    const long long rates = (long long)a.dim * N;
+    __shared__ float s_sum[16][kWave];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const long long i = (long long)(blockIdx.x - bc_blocks) * kWave + lane;
+    const long long rates = (long long)a.dim * N, columns = rates + 2 * a.dim;
+    const int parts = a.batch * g.segments, per = (parts + 15) / 16;
+    const int p0 = wave * per, p1 = p0 + per < parts ? p0 + per : parts;
+    float s = 0.f;
+    if (i < columns) {
+        const float *p = i < rates ? in.A + i : in.D + (i - rates);
+        const size_t step = i < rates ? (size_t)rates : (size_t)2 * a.dim;
+#pragma unroll 8
+        for (int q = p0; q < p1; ++q) s += p[(size_t)q * step];
+    }
+    s_sum[wave][lane] = s;
+    __syncthreads();
+    if (wave != 0 || i >= columns) return;
+    s = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) s += s_sum[w][lane];
     if (i < rates) {
-        float s = 0.f;
-        for (int p = 0; p < parts; ++p) s += in.A[(size_t)p * rates + i];
         a.grad_A[i] = s;
-    } else if (i < rates + 2 * a.dim) {
+    } else {
         const long long k = i - rates;
-        float s = 0.f;
-        for (int p = 0; p < parts; ++p) s += in.D[(size_t)p * 2 * a.dim + k];
         float *o = k < a.dim ? a.grad_D : a.grad_dt_bias;
         if (o) o[k < a.dim ? k : k - a.dim] = s;
     }
@@ -937,8 +961,9 @@ inline bool scan_shape_ok(int batch, int length, int dim, int state) {
 inline ScanGeom scan_geometry(int batch, int length, int dim) {
     ScanGeom g = {};
     g.groups = groups_of(dim);
+    g.padded = (length + kChunk - 1) / kChunk * kChunk;
     const long long waves = (long long)batch * g.groups;
-    long long want = waves >= 1024 ? 1 : (2048 + waves - 1) / waves;
+    long long want = waves >= 2048 ? 1 : (6144 + waves - 1) / waves;
     int len = (int)((length + want - 1) / want);
     if (len < 64) len = 64;
     g.seg_len = (len + kChunk - 1) / kChunk * kChunk;
@@ -946,8 +971,17 @@ inline ScanGeom scan_geometry(int batch, int length, int dim) {
     return g;
 }
 
+inline size_t rows_bytes(const ScanGeom &g, int batch, int state) {
+    return ((size_t)batch * g.padded + 1) * 2 * state * sizeof(float);
+}
+inline size_t chunk_bytes(const ScanGeom &g, int batch, int dim, int state) {
+    return (size_t)batch * (g.padded / kChunk) * dim * state * sizeof(float);
+}
+
+// The workspace of a forward call without chunk_states begins with the rows of B and C; with chunk_states they stand behind
+// the states there, where the backward call finds them.
 struct ScanSpace {
-    size_t seg_state, seg_delta, BC, A, D, total;
+    size_t rows, seg_state, seg_delta, BC, A, D, total;
 };
 inline ScanSpace scan_space(const ScanGeom &g, int batch, int length, int dim, int state, bool backward) {
     ScanSpace s = {};
@@ -957,6 +991,7 @@ inline ScanSpace scan_space(const ScanGeom &g, int batch, int length, int dim, i
         at += round16(floats * sizeof(float));
         return here;
     };
+    if (!backward) s.rows = take(rows_bytes(g, batch, state) / sizeof(float));
     if (g.segments > 1) {
         s.seg_state = take((size_t)batch * g.segments * state * dim);
         s.seg_delta = take((size_t)batch * g.segments * dim);
@@ -984,11 +1019,14 @@ template <typename DT, int N>
 rnntStatus_t scan_forward(const rnntScan &a, hipStream_t st) {
     ScanGeom g = scan_geometry(a.batch, a.length, a.dim);
     const unsigned grid = (unsigned)((long long)a.batch * g.segments * g.groups);
+    const ScanSpace s = scan_space(g, a.batch, a.length, a.dim, N, false);
+    char *ws = static_cast<char *>(a.workspace);
+    g.rows = a.chunk_states ? a.chunk_states + chunk_bytes(g, a.batch, a.dim, N) / sizeof(float) : reinterpret_cast<float *>(ws + s.rows);
+    const long long values = ((long long)a.batch * g.padded + 1) * 2 * N;
+    hipLaunchKernelGGL((scan_rows_kernel<DT, N>), dim3((unsigned)((values + 255) / 256)), dim3(256), 0, st, a, g);
     if (g.segments > 1) {
-        const ScanSpace s = scan_space(g, a.batch, a.length, a.dim, N, false);
-        if (a.workspace == nullptr || !aligned16(a.workspace)) return RNNT_STATUS_INVALID_VALUE;
-        g.seg_state = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + s.seg_state);
-        g.seg_delta = reinterpret_cast<float *>(static_cast<char *>(a.workspace) + s.seg_delta);
+        g.seg_state = reinterpret_cast<float *>(ws + s.seg_state);
+        g.seg_delta = reinterpret_cast<float *>(ws + s.seg_delta);
         hipLaunchKernelGGL((scan_forward_kernel<DT, N, true>), dim3(grid), dim3(64), 0, st, a, g);
         launch_join<N, false>(a, g, st);
     }
@@ -1001,6 +1039,7 @@ rnntStatus_t scan_backward(const rnntScan &a, hipStream_t st) {
     ScanGeom g = scan_geometry(a.batch, a.length, a.dim);
     const ScanSpace s = scan_space(g, a.batch, a.length, a.dim, N, true);
     char *ws = static_cast<char *>(a.workspace);
+    g.rows = const_cast<float *>(a.chunk_states) + chunk_bytes(g, a.batch, a.dim, N) / sizeof(float);
     const unsigned grid = (unsigned)((long long)a.batch * g.segments * g.groups);
     if (g.segments > 1) {
         g.seg_state = reinterpret_cast<float *>(ws + s.seg_state);
@@ -1011,9 +1050,9 @@ rnntStatus_t scan_backward(const rnntScan &a, hipStream_t st) {
     const ScanPartials p = {reinterpret_cast<float *>(ws + s.BC), reinterpret_cast<float *>(ws + s.A),
                             reinterpret_cast<float *>(ws + s.D)};
     hipLaunchKernelGGL((scan_backward_kernel<DT, N>), dim3(grid), dim3(N * 16), 0, st, a, g, p);
-    const unsigned bc = (unsigned)(((long long)a.batch * a.length * 2 * N + 255) / 256);
-    const unsigned pa = (unsigned)(((long long)a.dim * (N + 2) + 255) / 256);
-    hipLaunchKernelGGL((scan_backward_sum_kernel<DT, N>), dim3(bc + pa), dim3(256), 0, st, a, g, p, bc);
+    const unsigned bc = (unsigned)(((long long)a.batch * a.length * 2 * N + 1023) / 1024);
+    const unsigned pa = (unsigned)(((long long)a.dim * (N + 2) + kWave - 1) / kWave);
+    hipLaunchKernelGGL((scan_backward_sum_kernel<DT, N>), dim3(bc + pa), dim3(1024), 0, st, a, g, p, bc);
     return launched();
 }
 
@@ -1103,7 +1142,8 @@ extern "C" {
 
 rnntStatus_t rnnt_selective_scan_states_size(int batch, int length, int dim, int state, size_t *size_bytes) {
     if (size_bytes == nullptr || !scan_shape_ok(batch, length, dim, state)) return RNNT_STATUS_INVALID_VALUE;
-    *size_bytes = (size_t)batch * ((length + kChunk - 1) / kChunk) * dim * state * sizeof(float);
+    const ScanGeom g = scan_geometry(batch, length, dim);
+    *size_bytes = chunk_bytes(g, batch, dim, state) + rows_bytes(g, batch, state);
     return RNNT_STATUS_SUCCESS;
 }
 
@@ -1114,7 +1154,8 @@ rnntStatus_t rnnt_selective_scan_workspace_size(int batch, int length, int dim, 
 }
 
 rnntStatus_t rnnt_selective_scan_forward(const rnntScan *scan) {
-    if (!scan_args_ok(scan) || scan->y == nullptr || (scan->chunk_states && !aligned16(scan->chunk_states)))
+    if (!scan_args_ok(scan) || scan->y == nullptr || !scan->workspace || !aligned16(scan->workspace) ||
+        (scan->chunk_states && !aligned16(scan->chunk_states)))
         return RNNT_STATUS_INVALID_VALUE;
     SCAN_DISPATCH(scan_forward);
 }

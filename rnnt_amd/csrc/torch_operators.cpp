@@ -344,7 +344,7 @@ Tensor scan_workspace(const rnntScan &a, int backward, const Tensor &x) {
     size_t need = 0;
     check_status(rnnt_selective_scan_workspace_size(a.batch, a.length, a.dim, a.state, backward, &need),
                  "rnnt_selective_scan_workspace_size");
-    return need ? bytes(need, x) : Tensor();
+    return bytes(need, x);
 }
 
 std::tuple<Tensor, Tensor, Tensor> scan_forward(const ScanIn &in, bool keep) {

@@ -237,12 +237,13 @@ def test_c_entry_points_refuse_before_any_launch():
     scan = dict(batch=2, length=3, dim=4, state=16, x=16, dt=16, A=16, B=16, C=16, y=16, initial_state=16, final_state=16,
                 chunk_states=16, grad_y=16, grad_x=16, grad_dt=16, grad_A=16, grad_B=16, grad_C=16, workspace=16)
     for fn, change in ((lib.rnnt_selective_scan_forward, dict(state=12)), (lib.rnnt_selective_scan_forward, dict(A=None)),
-                       (lib.rnnt_selective_scan_forward, dict(chunk_states=8)), (lib.rnnt_selective_scan_forward, dict(dtype=-1)),
+                       (lib.rnnt_selective_scan_forward, dict(chunk_states=8)), (lib.rnnt_selective_scan_forward, dict(workspace=None)), (lib.rnnt_selective_scan_forward, dict(dtype=-1)),
                        (lib.rnnt_selective_scan_backward, dict(chunk_states=None)), (lib.rnnt_selective_scan_backward, dict(z=16)),
                        (lib.rnnt_selective_scan_backward, dict(workspace=None)), (lib.rnnt_selective_scan_step, dict(final_state=None)),
                        (lib.rnnt_selective_scan_step, dict(initial_state=None))):
         assert fn(ctypes.byref(_lib.RnntScan(**{**scan, **change}))) == 2, change
-    assert lib.rnnt_selective_scan_states_size(2, 33, 5, 16, ctypes.byref(n)) == 0 and n.value == 2 * 3 * 5 * 16 * 4
+    assert lib.rnnt_selective_scan_states_size(2, 33, 5, 16, ctypes.byref(n)) == 0
+    assert n.value == (2 * 3 * 5 * 16 + (2 * 48 + 1) * 2 * 16) * 4   # states before steps 0, 16, 32; rows of B and C
     assert lib.rnnt_selective_scan_states_size(1 << 20, 1 << 20, 64, 16, ctypes.byref(n)) == 2
 
 
