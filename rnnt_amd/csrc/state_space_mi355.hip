@@ -122,10 +122,29 @@ __global__ __launch_bounds__(256) void scan_rows_kernel(const rnntScan a, const 
     g.rows[i] = v;
 }
 
+// N adjacent floats at any address (16-byte loads need no more than 4-byte alignment)
+typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+template <int N>
+__device__ __forceinline__ void load_row(const float *p, float (&v)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; n += 4) {
+        const f32x4_any w = *reinterpret_cast<const f32x4_any *>(p + n);
+        v[n] = w.x;
+        v[n + 1] = w.y;
+        v[n + 2] = w.z;
+        v[n + 3] = w.w;
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_row(float *p, const float (&v)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; n += 4) *reinterpret_cast<f32x4_any *>(p + n) = f32x4_any{v[n], v[n + 1], v[n + 2], v[n + 3]};
+}
 template <int N>
 __device__ __forceinline__ void load_rates(const float *A, int d, float (&A2)[N]) {
+    load_row<N>(A + (size_t)d * N, A2);
 #pragma unroll
-    for (int n = 0; n < N; ++n) A2[n] = A[(size_t)d * N + n] * kLog2e;
+    for (int n = 0; n < N; ++n) A2[n] *= kLog2e;
 }
 
 // state tiles between kernels: [N / 4][dim][4] per (sequence, time)
@@ -133,22 +152,16 @@ template <int N>
 __device__ __forceinline__ void load_tile(const float *tile, int dim, int d, float (&h)[N]) {
 #pragma unroll
     for (int q = 0; q < N / 4; ++q) {
-        const f32x2 *p = reinterpret_cast<const f32x2 *>(tile + ((size_t)q * dim + d) * 4);
-        const f32x2 lo = p[0], hi = p[1];
-        h[4 * q] = lo.x;
-        h[4 * q + 1] = lo.y;
-        h[4 * q + 2] = hi.x;
-        h[4 * q + 3] = hi.y;
+        const f32x4 v = *reinterpret_cast<const f32x4 *>(tile + ((size_t)q * dim + d) * 4);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) h[4 * q + n] = v[n];
     }
 }
 template <int N>
 __device__ __forceinline__ void store_tile(float *tile, int dim, int d, const float (&h)[N]) {
 #pragma unroll
-    for (int q = 0; q < N / 4; ++q) {
-        f32x2 *p = reinterpret_cast<f32x2 *>(tile + ((size_t)q * dim + d) * 4);
-        p[0] = f32x2{h[4 * q], h[4 * q + 1]};
-        p[1] = f32x2{h[4 * q + 2], h[4 * q + 3]};
-    }
+    for (int q = 0; q < N / 4; ++q)
+        *reinterpret_cast<f32x4 *>(tile + ((size_t)q * dim + d) * 4) = f32x4{h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]};
 }
 
 // One wave walks 64 channels of one segment; lane = channel, all N states of it in registers.
@@ -178,8 +191,7 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
         if (seg_state) {
             load_tile<N>(seg_state, a.dim, d, h);
         } else if (a.initial_state) {
-#pragma unroll
-            for (int n = 0; n < N; ++n) h[n] = a.initial_state[((size_t)b * a.dim + d) * N + n];
+            load_row<N>(a.initial_state + ((size_t)b * a.dim + d) * N, h);
         }
     }
     const float skip = !LOCAL && a.D ? a.D[d] : 0.f;
@@ -266,43 +278,69 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
         for (int t = te; t < t1; ++t) yp[(size_t)t * a.dim] = DT::from_float(0.f);
         // the segment that holds the last step (segment 0 of an empty sequence) has the final state
         const bool last = len > t0 ? len <= t1 : (seg == 0 && len == 0);
-        if (a.final_state && last) {
-#pragma unroll
-            for (int n = 0; n < N; ++n) a.final_state[((size_t)b * a.dim + d) * N + n] = h[n];
-        }
+        if (a.final_state && last) store_row<N>(a.final_state + ((size_t)b * a.dim + d) * N, h);
     }
 }
 
 // Pass 2: the state (forward) or the state's gradient (backward) at every segment's border, in order.
 //   forward:  seg_state[s] <- state before segment s;      state <- exp(A sum_delta[s]) state + end[s]
 //   backward: seg_state[s] <- gradient after segment s;    the same towards smaller s, the start grad_final
-// One thread per (sequence, channel, 4 states).
+// A lane has 4 states of a channel.  The waves of a workgroup share the segments: each joins its range from zero, which
+// gives a decay and an end for the range, and walks it again from what the ranges before it give.  Loads of kJoinAhead
+// segments are under way at once: alone they are a chain of two loads and an exponential per segment.
+constexpr int kJoinWaves = 8, kJoinAhead = 8;
+
 template <int N, bool BACKWARD>
-__global__ __launch_bounds__(256) void scan_join_kernel(const rnntScan a, const ScanGeom g) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(kJoinWaves *kWave) void scan_join_kernel(const rnntScan a, const ScanGeom g) {
+    __shared__ float s_end[kJoinWaves][4][kWave], s_delta[kJoinWaves][kWave];
+    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+    const long long i = (long long)blockIdx.x * kWave + lane;
     const int d = (int)(i % a.dim);
     const long long r = i / a.dim;
     const int q = (int)(r % (N / 4));
     const long long b = r / (N / 4);
-    if (b >= a.batch) return;
+    const bool ok = b < a.batch;
+    const int per = (g.segments + kJoinWaves - 1) / kJoinWaves;
+    const int k0 = wave * per, k1 = !ok ? k0 : (k0 + per < g.segments ? k0 + per : g.segments);
     float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < 4; ++n) A2[n] = ok ? a.A[(size_t)d * N + q * 4 + n] * kLog2e : 0.f;
+    f32x4 *tiles = reinterpret_cast<f32x4 *>(g.seg_state) + ((size_t)b * g.segments * (N / 4) + q) * a.dim + d;
+    const float *deltas = g.seg_delta + (size_t)b * g.segments * a.dim + d;
+    auto walk = [&](bool write) {
+        float sum = 0.f;
+        for (int kb = k0; kb < k1; kb += kJoinAhead) {
+            f32x4 end[kJoinAhead];
+            float delta[kJoinAhead];
+#pragma unroll
+            for (int j = 0; j < kJoinAhead; ++j) {
+                const int k = kb + j < k1 ? kb + j : k1 - 1, s = BACKWARD ? g.segments - 1 - k : k;
+                end[j] = tiles[(size_t)s * (N / 4) * a.dim];
+                delta[j] = deltas[(size_t)s * a.dim];
+            }
+#pragma unroll
+            for (int j = 0; j < kJoinAhead; ++j) {
+                if (kb + j >= k1) break;
+                const int s = BACKWARD ? g.segments - 1 - (kb + j) : kb + j;
+                if (write) tiles[(size_t)s * (N / 4) * a.dim] = f32x4{h[0], h[1], h[2], h[3]};
+                sum += delta[j];
+#pragma unroll
+                for (int n = 0; n < 4; ++n) h[n] = fma_(exp2_(delta[j] * A2[n]), h[n], end[j][n]);
+            }
+        }
+        return sum;
+    };
+    s_delta[wave][lane] = walk(false);
+#pragma unroll
+    for (int n = 0; n < 4; ++n) s_end[wave][n][lane] = h[n];
+    __syncthreads();
     const float *from = BACKWARD ? a.grad_final : a.initial_state;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-        A2[n] = a.A[(size_t)d * N + q * 4 + n] * kLog2e;
-        if (from) h[n] = from[((size_t)b * a.dim + d) * N + q * 4 + n];
+        h[n] = from && ok ? from[((size_t)b * a.dim + d) * N + q * 4 + n] : 0.f;
+        for (int w = 0; w < wave; ++w) h[n] = fma_(exp2_(s_delta[w][lane] * A2[n]), h[n], s_end[w][n][lane]);
     }
-    for (int k = 0; k < g.segments; ++k) {
-        const int s = BACKWARD ? g.segments - 1 - k : k;
-        float *tile = g.seg_state + (((size_t)b * g.segments + s) * (N / 4) + q) * a.dim * 4 + (size_t)d * 4;
-        const float delta = g.seg_delta[((size_t)b * g.segments + s) * a.dim + d];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const float end = tile[n];
-            tile[n] = h[n];
-            h[n] = fma_(exp2_(delta * A2[n]), h[n], end);
-        }
-    }
+    walk(true);
 }
 
 // Pass 1 of the backward: the gradient of a segment's first state that its own outputs give.
@@ -420,8 +458,9 @@ __device__ __forceinline__ float lanes_sum(float (&v)[V], int lane) {
 }
 
 // The backward proper.  The N / 4 waves of a workgroup share 64 channels of one segment; wave w owns the states
-// [4 w, 4 w + 4) of all of them, so that a chunk of 16 steps of h and of exp(delta A) stays in registers (2 x 16 x 4)
-// and B, C stay scalar operands.  Per chunk, from the last to the first:
+// [4 w, 4 w + 4) of all of them, so that a chunk of 16 steps of h and of exp(delta A) stays in registers (2 x 16 x 4).
+// B and C come from LDS, 16 bytes at an address that the wave shares: scalar loads return out of order, so that each use
+// would wait for all of them.  Per chunk, from the last to the first:
 //   1. each wave turns its share of the steps' inputs into delta, x, gy (LDS), keeping what its outputs need;
 //   2. each wave walks its states forwards from the saved state, then backwards, summing dB, dC over the 64 lanes and
 //      leaving its share of the sums over n in LDS;
@@ -439,6 +478,7 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
     __shared__ float s_delta[kChunk][kWave], s_x[kChunk][kWave], s_gy[kChunk][kWave];
     __shared__ float s_part[3][W][kChunk][kWave];
     __shared__ float s_bc[kChunk][2 * N];
+    __shared__ f32x4 s_rows[kChunk][N / 2];
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int group = blockIdx.x % g.groups;
@@ -478,7 +518,7 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
     const E *zp = gated ? static_cast<const E *>(a.z) + b * a.z_batch + d : xp;
     const long long z_time = gated ? a.z_time : a.x_time;
     const E *gp = static_cast<const E *>(a.grad_y) + b * a.grad_y_batch + d;
-    const float *rows = g.rows + (size_t)b * g.padded * 2 * N + wave * 2 * S;
+    const f32x2 *rows = reinterpret_cast<const f32x2 *>(g.rows + (size_t)b * g.padded * 2 * N) + threadIdx.x;
     const size_t out0 = (size_t)b * a.length * a.dim + d;
     E *dxp = static_cast<E *>(a.grad_x) + out0, *ddtp = static_cast<E *>(a.grad_dt) + out0;
     E *dzp = gated ? static_cast<E *>(a.grad_z) + out0 : nullptr;
@@ -494,6 +534,7 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
     // a chunk's inputs are under way while the chunk after it is computed
     E xn[kMine], dtn[kMine], zn[kMine], gn[kMine];
     f32x4 hn;
+    f32x2 rn;
     auto fetch = [&](int c) {
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
@@ -504,6 +545,7 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
             zn[j] = zp[tt * z_time];
             gn[j] = gp[tt * a.grad_y_time];
         }
+        rn = rows[(size_t)c * (kChunk * N)];  // (two values per thread are a chunk's rows)
         hn = *reinterpret_cast<const f32x4 *>(a.chunk_states + ((size_t)b * chunks + c) * N * a.dim + ((size_t)wave * a.dim + d) * 4);
     };
     const int c0 = t0 / kChunk;
@@ -528,6 +570,7 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
             s_x[i][lane] = in ? x : 0.f;
             s_gy[i][lane] = in ? gy : 0.f;
         }
+        reinterpret_cast<f32x2 *>(s_rows)[threadIdx.x] = rn;
         float h[S] = {hn.x, hn.y, hn.z, hn.w};
         if (c > c0) fetch(c - 1);
         __syncthreads();
@@ -535,32 +578,30 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
         float before[kChunk][S], decay[kChunk][S];
 #pragma unroll
         for (int i = 0; i < kChunk; ++i) {
-            ScalarRow<S> row;
-            row.load(rows + (size_t)(tc + i) * 2 * N);
+            const f32x4 B = s_rows[i][2 * wave], C = s_rows[i][2 * wave + 1];
             const float delta = s_delta[i][lane], dx = delta * s_x[i][lane];
             float y = 0.f;
 #pragma unroll
             for (int n = 0; n < S; ++n) {
                 before[i][n] = h[n];
                 decay[i][n] = exp2_(delta * A2[n]);
-                h[n] = fma_(decay[i][n], h[n], dx * row.B(n));
-                y = fma_(row.C(n), h[n], y);
+                h[n] = fma_(decay[i][n], h[n], dx * B[n]);
+                y = fma_(C[n], h[n], y);
             }
             s_part[0][wave][i][lane] = y;
         }
 #pragma unroll
         for (int i = kChunk - 1; i >= 0; --i) {
-            ScalarRow<S> row;
-            row.load(rows + (size_t)(tc + i) * 2 * N);
+            const f32x4 B = s_rows[i][2 * wave], C = s_rows[i][2 * wave + 1];
             const float delta = s_delta[i][lane], dx = delta * s_x[i][lane], gy = s_gy[i][lane];
             float inner = 0.f, rate = 0.f, sums[2 * S];
 #pragma unroll
             for (int n = 0; n < S; ++n) {
                 const float after = i + 1 < kChunk ? before[i + 1 < kChunk ? i + 1 : 0][n] : h[n];
-                const float gn = fma_(row.C(n), gy, G[n]);
+                const float gn = fma_(C[n], gy, G[n]);
                 sums[n] = gn * dx;
                 sums[S + n] = after * gy;
-                inner = fma_(gn, row.B(n), inner);
+                inner = fma_(gn, B[n], inner);
                 G[n] = gn * decay[i][n];
                 const float r = G[n] * before[i][n];
                 dA[n] = fma_(r, delta, dA[n]);
@@ -1012,7 +1053,8 @@ inline bool scan_args_ok(const rnntScan *a) {
 template <int N, bool BACKWARD>
 void launch_join(const rnntScan &a, const ScanGeom &g, hipStream_t st) {
     const long long n = (long long)a.batch * a.dim * (N / 4);
-    hipLaunchKernelGGL((scan_join_kernel<N, BACKWARD>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a, g);
+    hipLaunchKernelGGL((scan_join_kernel<N, BACKWARD>), dim3((unsigned)((n + kWave - 1) / kWave)), dim3(kJoinWaves * kWave), 0, st, a,
+                       g);
 }
 
 template <typename DT, int N>
