@@ -92,6 +92,8 @@ struct ScanGeom {
     int groups;    // of 64 channels
     int segments;  // per sequence
     int seg_len;   // steps per segment, a multiple of kChunk
+    int blocks;    // per sequence: what a workgroup of the backward proper takes, `joined` segments each
+    int joined;
     float *seg_state;  // [batch][segments][state / 4][dim][4]: a segment's end from zero, then the state it starts from
     float *seg_delta;  // [batch][segments][dim]: sum of delta over the segment
     float *rows;       // B and C: [batch][length rounded up to kChunk][2 state], and one row more
@@ -152,7 +154,7 @@ template <int N>
 __device__ __forceinline__ void load_tile(const float *tile, int dim, int d, float (&h)[N]) {
 #pragma unroll
     for (int q = 0; q < N / 4; ++q) {
-        const f32x4 v = *reinterpret_cast<const f32x4 *>(tile + ((size_t)q * dim + d) * 4);
+        const f32x4 v = reinterpret_cast<const f32x4 *>(tile + (size_t)q * dim * 4)[(unsigned)d];
 #pragma unroll
         for (int n = 0; n < 4; ++n) h[4 * q + n] = v[n];
     }
@@ -161,7 +163,7 @@ template <int N>
 __device__ __forceinline__ void store_tile(float *tile, int dim, int d, const float (&h)[N]) {
 #pragma unroll
     for (int q = 0; q < N / 4; ++q)
-        *reinterpret_cast<f32x4 *>(tile + ((size_t)q * dim + d) * 4) = f32x4{h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]};
+        reinterpret_cast<f32x4 *>(tile + (size_t)q * dim * 4)[(unsigned)d] = f32x4{h[4 * q], h[4 * q + 1], h[4 * q + 2], h[4 * q + 3]};
 }
 
 // One wave walks 64 channels of one segment; lane = channel, all N states of it in registers.
@@ -176,6 +178,7 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
     const int d0 = group * kWave + lane;
     const bool ok = d0 < a.dim;
     const int d = ok ? d0 : a.dim - 1;
+    const unsigned lo = d;  // (a lane's offset from an address that the wave shares)
     const int t0 = seg * g.seg_len;
     const int t1 = t0 + g.seg_len < a.length ? t0 + g.seg_len : a.length;
     const int len = clamp_len(a.lengths, b, a.length);
@@ -195,13 +198,13 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
         }
     }
     const float skip = !LOCAL && a.D ? a.D[d] : 0.f;
-    const E *xp = static_cast<const E *>(a.x) + b * a.x_batch + d;
-    const E *dtp = static_cast<const E *>(a.dt) + b * a.dt_batch + d;
+    const E *xp = static_cast<const E *>(a.x) + b * a.x_batch;
+    const E *dtp = static_cast<const E *>(a.dt) + b * a.dt_batch;
     const bool gated = a.z != nullptr;  // (without a gate its loads repeat x's: no branch between loads)
-    const E *zp = gated ? static_cast<const E *>(a.z) + b * a.z_batch + d : xp;
+    const E *zp = gated ? static_cast<const E *>(a.z) + b * a.z_batch : xp;
     const long long z_time = gated ? a.z_time : a.x_time;
     const float *rows = g.rows + ((size_t)b * g.padded + t0) * 2 * N;
-    E *yp = LOCAL ? nullptr : static_cast<E *>(a.y) + (size_t)b * a.length * a.dim + d;
+    E *yp = LOCAL ? nullptr : static_cast<E *>(a.y) + (size_t)b * a.length * a.dim;
     const int chunks = (a.length + kChunk - 1) / kChunk;
     float sum_delta = 0.f;
 
@@ -210,9 +213,9 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const long long tt = t + j < te ? t + j : te - 1;
-            xn[j] = xp[tt * a.x_time];
-            dtn[j] = dtp[tt * a.dt_time];
-            if (!LOCAL) zn[j] = zp[tt * z_time];
+            xn[j] = (xp + tt * a.x_time)[lo];
+            dtn[j] = (dtp + tt * a.dt_time)[lo];
+            if (!LOCAL) zn[j] = (zp + tt * z_time)[lo];
         }
     };
     // the next step's row is under way while a step is computed (32 states of two rows would not fit the scalar registers)
@@ -263,7 +266,7 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
                     const float z = DT::to_float(zc[j]);
                     y *= z * sigmoid_(z);
                 }
-                if (ok) yp[(size_t)t * a.dim] = DT::from_float(y);
+                if (ok) (yp + (size_t)t * a.dim)[lo] = DT::from_float(y);
             }
         }
     }
@@ -275,7 +278,7 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
         return;
     }
     if (ok) {
-        for (int t = te; t < t1; ++t) yp[(size_t)t * a.dim] = DT::from_float(0.f);
+        for (int t = te; t < t1; ++t) (yp + (size_t)t * a.dim)[lo] = DT::from_float(0.f);
         // the segment that holds the last step (segment 0 of an empty sequence) has the final state
         const bool last = len > t0 ? len <= t1 : (seg == 0 && len == 0);
         if (a.final_state && last) store_row<N>(a.final_state + ((size_t)b * a.dim + d) * N, h);
@@ -288,11 +291,12 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
 // A lane has 4 states of a channel.  The waves of a workgroup share the segments: each joins its range from zero, which
 // gives a decay and an end for the range, and walks it again from what the ranges before it give.  Loads of kJoinAhead
 // segments are under way at once: alone they are a chain of two loads and an exponential per segment.
+// Up to kJoinAhead segments one wave does it alone, once.
 constexpr int kJoinWaves = 8, kJoinAhead = 8;
 
-template <int N, bool BACKWARD>
-__global__ __launch_bounds__(kJoinWaves *kWave) void scan_join_kernel(const rnntScan a, const ScanGeom g) {
-    __shared__ float s_end[kJoinWaves][4][kWave], s_delta[kJoinWaves][kWave];
+template <int N, bool BACKWARD, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave) void scan_join_kernel(const rnntScan a, const ScanGeom g) {
+    __shared__ float s_end[WAVES][4][kWave], s_delta[WAVES][kWave];
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const long long i = (long long)blockIdx.x * kWave + lane;
     const int d = (int)(i % a.dim);
@@ -300,7 +304,7 @@ __global__ __launch_bounds__(kJoinWaves *kWave) void scan_join_kernel(const rnnt
     const int q = (int)(r % (N / 4));
     const long long b = r / (N / 4);
     const bool ok = b < a.batch;
-    const int per = (g.segments + kJoinWaves - 1) / kJoinWaves;
+    const int per = (g.segments + WAVES - 1) / WAVES;
     const int k0 = wave * per, k1 = !ok ? k0 : (k0 + per < g.segments ? k0 + per : g.segments);
     float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -330,10 +334,12 @@ __global__ __launch_bounds__(kJoinWaves *kWave) void scan_join_kernel(const rnnt
         }
         return sum;
     };
-    s_delta[wave][lane] = walk(false);
+    if (WAVES > 1) {
+        s_delta[wave][lane] = walk(false);
 #pragma unroll
-    for (int n = 0; n < 4; ++n) s_end[wave][n][lane] = h[n];
-    __syncthreads();
+        for (int n = 0; n < 4; ++n) s_end[wave][n][lane] = h[n];
+        __syncthreads();
+    }
     const float *from = BACKWARD ? a.grad_final : a.initial_state;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
@@ -355,6 +361,7 @@ __global__ __launch_bounds__(64) void scan_backward_local_kernel(const rnntScan 
     const int d0 = group * kWave + lane;
     const bool ok = d0 < a.dim;
     const int d = ok ? d0 : a.dim - 1;
+    const unsigned lo = d;  // (a lane's offset from an address that the wave shares)
     const int t0 = seg * g.seg_len;
     const int t1 = t0 + g.seg_len < a.length ? t0 + g.seg_len : a.length;
     const int len = clamp_len(a.lengths, b, a.length);
@@ -365,11 +372,11 @@ __global__ __launch_bounds__(64) void scan_backward_local_kernel(const rnntScan 
 #pragma unroll
     for (int n = 0; n < N; ++n) G[n] = 0.f;
     const float bias = a.dt_bias ? a.dt_bias[d] : 0.f;
-    const E *dtp = static_cast<const E *>(a.dt) + b * a.dt_batch + d;
+    const E *dtp = static_cast<const E *>(a.dt) + b * a.dt_batch;
     const bool gated = a.z != nullptr;
-    const E *zp = gated ? static_cast<const E *>(a.z) + b * a.z_batch + d : dtp;
+    const E *zp = gated ? static_cast<const E *>(a.z) + b * a.z_batch : dtp;
     const long long z_time = gated ? a.z_time : a.dt_time;
-    const E *gp = static_cast<const E *>(a.grad_y) + b * a.grad_y_batch + d;
+    const E *gp = static_cast<const E *>(a.grad_y) + b * a.grad_y_batch;
     const float *rows = g.rows + ((size_t)b * g.padded + te) * 2 * N;  // one past the step
     float sum_delta = 0.f;
     E dtn[kAhead], zn[kAhead], gn[kAhead];
@@ -377,9 +384,9 @@ __global__ __launch_bounds__(64) void scan_backward_local_kernel(const rnntScan 
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const long long tt = t - j > t0 ? t - j : t0;
-            dtn[j] = dtp[tt * a.dt_time];
-            gn[j] = gp[tt * a.grad_y_time];
-            zn[j] = zp[tt * z_time];
+            dtn[j] = (dtp + tt * a.dt_time)[lo];
+            gn[j] = (gp + tt * a.grad_y_time)[lo];
+            zn[j] = (zp + tt * z_time)[lo];
         }
     };
     if (te > t0) fetch(te - 1);
@@ -417,45 +424,59 @@ __global__ __launch_bounds__(64) void scan_backward_local_kernel(const rnntScan 
     }
 }
 
-// ---- sums over the 64 lanes of V values at once --------------------------------------------------------------------
-// Every step halves the values and the lanes that share one: 2 V instructions instead of 6 V.  Afterwards lane l holds
-// the sum of value l / (64 / V).
+// ---- sums over the 64 lanes ------------------------------------------------------------------------------------------
+// 8 values of each of 8 steps are summed over the lanes as one tree: every stage halves the values and the lanes that
+// share one, 18 instructions a step where 8 separate butterflies would take 48.
 template <int CTRL>
 __device__ __forceinline__ float dpp_(float v) {
     return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CTRL, 0xf, 0xf, true));
 }
 constexpr int kQuadXor1 = 0xB1, kQuadXor2 = 0x4E, kHalfMirror = 0x141, kRowRor8 = 0x128;
 
-template <int V>
-__device__ __forceinline__ float lanes_sum(float (&v)[V], int lane) {
-    static_assert(V == 4 || V == 8 || V == 16, "");
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + V / 2]), false, false);
-        v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-#pragma unroll
-    for (int i = 0; i < V / 4; ++i) {
-        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + V / 4]), false, false);
-        v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-    }
-    if constexpr (V >= 8) {
-        const bool up = lane & 8;
-#pragma unroll
-        for (int i = 0; i < V / 8; ++i) v[i] = (up ? v[i + V / 8] : v[i]) + dpp_<kRowRor8>(up ? v[i] : v[i + V / 8]);
-    } else {
-        v[0] += dpp_<kRowRor8>(v[0]);
-    }
-    if constexpr (V >= 16) {
-        const bool up = lane & 4;
-        v[0] = (up ? v[1] : v[0]) + dpp_<kHalfMirror>(up ? v[0] : v[1]);
-    } else {
-        v[0] += dpp_<kHalfMirror>(v[0]);
-    }
-    v[0] += dpp_<kQuadXor2>(v[0]);
-    v[0] += dpp_<kQuadXor1>(v[0]);
-    return v[0];
+// lanes without `up` keep a's sums, the others b's; CTRL exchanges the two kinds of lanes
+template <int CTRL>
+__device__ __forceinline__ float fold(float a, float b, bool up) {
+    return (up ? b : a) + dpp_<CTRL>(up ? a : b);
 }
+
+// 8 values over the lane bits 5, 4, 3: lane l then has the sums of value l / 8 over 8 of the 64 lanes
+__device__ __forceinline__ float fold_values(float (&v)[8], int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 4]), false, false);
+        v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 2]), false, false);
+        v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return fold<kRowRor8>(v[0], v[1], lane & 8);
+}
+
+// The steps of a chunk, taken from the last to the first, over the lane bits 2, 1, 0: when step 8 j comes, lane l gets the
+// sums of step 8 j + (l >> 2 & 1) + 2 (l >> 1 & 1) + 4 (l & 1).
+struct FoldSteps {
+    float held[3];
+    template <int I>
+    __device__ __forceinline__ float take(float v, int lane) {
+        if constexpr (I & 1) {
+            held[0] = v;
+        } else {
+            v = fold<kHalfMirror>(v, held[0], lane & 4);
+            if constexpr (I & 2) {
+                held[1] = v;
+            } else {
+                v = fold<kQuadXor2>(v, held[1], lane & 2);
+                if constexpr (I & 4)
+                    held[2] = v;
+                else
+                    v = fold<kQuadXor1>(v, held[2], lane & 1);
+            }
+        }
+        return v;
+    }
+};
 
 // The backward proper.  The N / 4 waves of a workgroup share 64 channels of one segment; wave w owns the states
 // [4 w, 4 w + 4) of all of them, so that a chunk of 16 steps of h and of exp(delta A) stays in registers (2 x 16 x 4).
@@ -465,10 +486,22 @@ __device__ __forceinline__ float lanes_sum(float (&v)[V], int lane) {
 //   2. each wave walks its states forwards from the saved state, then backwards, summing dB, dC over the 64 lanes and
 //      leaving its share of the sums over n in LDS;
 //   3. each wave adds the waves' shares of its steps and writes dx, ddt, dz.
+template <int I>
+struct Index {
+    static constexpr int value = I;
+};
+template <int I, typename F>
+__device__ __forceinline__ void down(F &&f) {  // f at I - 1, I - 2, ..., 0, each a constant
+    if constexpr (I > 0) {
+        f(Index<I - 1>());
+        down<I - 1>(f);
+    }
+}
+
 struct ScanPartials {
     float *BC;      // [batch][length][groups][2 N]
-    float *A;       // [batch * segments][dim * N]
-    float *D;       // [batch * segments][2][dim]: D, dt_bias
+    float *A;       // [batch * blocks][dim * N]
+    float *D;       // [batch * blocks][2][dim]: D, dt_bias
 };
 
 template <typename DT, int N>
@@ -483,12 +516,13 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int group = blockIdx.x % g.groups;
     const int rest = blockIdx.x / g.groups;
-    const int seg = rest % g.segments, b = rest / g.segments;
+    const int block = rest % g.blocks, b = rest / g.blocks;
     const int d0 = group * kWave + lane;
     const bool ok = d0 < a.dim;
     const int d = ok ? d0 : a.dim - 1;
-    const int t0 = seg * g.seg_len;
-    const int t1 = t0 + g.seg_len < a.length ? t0 + g.seg_len : a.length;
+    const unsigned lo = d;  // (a lane's offset from an address that the wave shares)
+    const int steps_per = g.joined * g.seg_len, t0 = block * steps_per;
+    const int t1 = t0 + steps_per < a.length ? t0 + steps_per : a.length;
     const int len = clamp_len(a.lengths, b, a.length);
     const int te = len < t1 ? (len > t0 ? len : t0) : t1;
     const int chunks = (a.length + kChunk - 1) / kChunk;
@@ -503,7 +537,8 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
     // (states of 4 to a tile row: state n of the layer is element n % 4 of row n / 4)
     auto tile_at = [&](const float *tile, int n) { return tile + ((size_t)(n / 4) * a.dim + d) * 4 + n % 4; };
     if (g.segments > 1) {
-        const float *tile = g.seg_state + ((size_t)b * g.segments + seg) * N * a.dim;
+        const int last = block < g.blocks - 1 ? (block + 1) * g.joined - 1 : g.segments - 1;
+        const float *tile = g.seg_state + ((size_t)b * g.segments + last) * N * a.dim;
 #pragma unroll
         for (int n = 0; n < S; ++n) G[n] = *tile_at(tile, wave * S + n);
     } else if (a.grad_final) {
@@ -512,23 +547,23 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
     }
     const float bias = a.dt_bias ? a.dt_bias[d] : 0.f;
     const float skip = a.D ? a.D[d] : 0.f;
-    const E *xp = static_cast<const E *>(a.x) + b * a.x_batch + d;
-    const E *dtp = static_cast<const E *>(a.dt) + b * a.dt_batch + d;
+    const E *xp = static_cast<const E *>(a.x) + b * a.x_batch;
+    const E *dtp = static_cast<const E *>(a.dt) + b * a.dt_batch;
     const bool gated = a.z != nullptr;
-    const E *zp = gated ? static_cast<const E *>(a.z) + b * a.z_batch + d : xp;
+    const E *zp = gated ? static_cast<const E *>(a.z) + b * a.z_batch : xp;
     const long long z_time = gated ? a.z_time : a.x_time;
-    const E *gp = static_cast<const E *>(a.grad_y) + b * a.grad_y_batch + d;
+    const E *gp = static_cast<const E *>(a.grad_y) + b * a.grad_y_batch;
     const f32x2 *rows = reinterpret_cast<const f32x2 *>(g.rows + (size_t)b * g.padded * 2 * N) + threadIdx.x;
-    const size_t out0 = (size_t)b * a.length * a.dim + d;
+    const size_t out0 = (size_t)b * a.length * a.dim;
     E *dxp = static_cast<E *>(a.grad_x) + out0, *ddtp = static_cast<E *>(a.grad_dt) + out0;
     E *dzp = gated ? static_cast<E *>(a.grad_z) + out0 : nullptr;
     float dD = 0.f, dbias = 0.f;
 
     if (ok) {
         for (int t = te + wave; t < t1; t += W) {
-            dxp[(size_t)t * a.dim] = DT::from_float(0.f);
-            ddtp[(size_t)t * a.dim] = DT::from_float(0.f);
-            if (dzp) dzp[(size_t)t * a.dim] = DT::from_float(0.f);
+            (dxp + (size_t)t * a.dim)[lo] = DT::from_float(0.f);
+            (ddtp + (size_t)t * a.dim)[lo] = DT::from_float(0.f);
+            if (dzp) (dzp + (size_t)t * a.dim)[lo] = DT::from_float(0.f);
         }
     }
     // a chunk's inputs are under way while the chunk after it is computed
@@ -540,13 +575,13 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
         for (int j = 0; j < kMine; ++j) {
             const int t = c * kChunk + wave * kMine + j;
             const long long tt = t < te ? t : te - 1;
-            xn[j] = xp[tt * a.x_time];
-            dtn[j] = dtp[tt * a.dt_time];
-            zn[j] = zp[tt * z_time];
-            gn[j] = gp[tt * a.grad_y_time];
+            xn[j] = (xp + tt * a.x_time)[lo];
+            dtn[j] = (dtp + tt * a.dt_time)[lo];
+            zn[j] = (zp + tt * z_time)[lo];
+            gn[j] = (gp + tt * a.grad_y_time)[lo];
         }
         rn = rows[(size_t)c * (kChunk * N)];  // (two values per thread are a chunk's rows)
-        hn = *reinterpret_cast<const f32x4 *>(a.chunk_states + ((size_t)b * chunks + c) * N * a.dim + ((size_t)wave * a.dim + d) * 4);
+        hn = reinterpret_cast<const f32x4 *>(a.chunk_states + ((size_t)b * chunks + c) * N * a.dim + (size_t)wave * a.dim * 4)[lo];
     };
     const int c0 = t0 / kChunk;
     if (te > t0) fetch((te - 1) / kChunk);
@@ -590,8 +625,10 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
             }
             s_part[0][wave][i][lane] = y;
         }
-#pragma unroll
-        for (int i = kChunk - 1; i >= 0; --i) {
+        FoldSteps steps;
+        float sums_of[kChunk / 8];
+        auto reverse = [&](auto index) {
+            constexpr int i = decltype(index)::value;
             const f32x4 B = s_rows[i][2 * wave], C = s_rows[i][2 * wave + 1];
             const float delta = s_delta[i][lane], dx = delta * s_x[i][lane], gy = s_gy[i][lane];
             float inner = 0.f, rate = 0.f, sums[2 * S];
@@ -609,11 +646,19 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
             }
             s_part[1][wave][i][lane] = inner;
             s_part[2][wave][i][lane] = rate;
+            const float sum = steps.template take<i>(fold_values(sums, lane), lane);
+            if constexpr (i % 8 == 0) sums_of[i / 8] = sum;
+            // (a scheduler free to mix steps, or to put dA's additions off, wants more than the 256 registers that two waves
+            // per SIMD leave)
+#pragma unroll
+            for (int n = 0; n < S; ++n) asm volatile("" : "+v"(dA[n]));
             __builtin_amdgcn_sched_barrier(0);
-            const float sum = lanes_sum<2 * S>(sums, lane);
-            constexpr int kShare = kWave / (2 * S);
-            const int k = lane / kShare;
-            if (lane % kShare == 0) s_bc[i][(k < S ? 0 : N - S) + wave * S + k] = sum;
+        };
+        down<kChunk>(reverse);
+        {
+            const int k = lane >> 3, i = (lane >> 2 & 1) + (lane & 2) + (lane & 1) * 4;
+#pragma unroll
+            for (int j = 0; j < kChunk / 8; ++j) s_bc[8 * j + i][(k < S ? 0 : N - S) + wave * S + k] = sums_of[j];
         }
         __syncthreads();
 
@@ -630,25 +675,27 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
             const float delta = s_delta[i][lane], x = s_x[i][lane], gy = s_gy[i][lane];
             if (t < te && ok) {
                 const float ddt = fma_(x, inner, rate * kLn2) * sigv[j];
-                dxp[(size_t)t * a.dim] = DT::from_float(fma_(delta, inner, skip * gy));
-                ddtp[(size_t)t * a.dim] = DT::from_float(ddt);
-                if (dzp) dzp[(size_t)t * a.dim] = DT::from_float(dzf[j] * fma_(skip, x, y));
+                (dxp + (size_t)t * a.dim)[lo] = DT::from_float(fma_(delta, inner, skip * gy));
+                (ddtp + (size_t)t * a.dim)[lo] = DT::from_float(ddt);
+                if (dzp) (dzp + (size_t)t * a.dim)[lo] = DT::from_float(dzf[j] * fma_(skip, x, y));
                 dD = fma_(gy, x, dD);
                 dbias += ddt;
             }
         }
-        for (int k = threadIdx.x; k < kChunk * 2 * N; k += W * kWave) {
-            const int i = k / (2 * N), t = tc + i;
-            if (t < te) out.BC[(((size_t)b * a.length + t) * g.groups + group) * 2 * N + k % (2 * N)] = s_bc[i][k % (2 * N)];
+        {  // two values per thread are the chunk's shares of dB and dC
+            const int i = threadIdx.x / N, k = threadIdx.x % N;
+            if (tc + i < te)
+                *reinterpret_cast<f32x2 *>(out.BC + (((size_t)b * a.length + tc + i) * g.groups + group) * 2 * N + 2 * k) =
+                    *reinterpret_cast<const f32x2 *>(&s_bc[i][2 * k]);
         }
         __syncthreads();
     }
 
-    const size_t part = (size_t)b * g.segments + seg;
+    const size_t part = (size_t)b * g.blocks + block;
     if (ok) {
 #pragma unroll
         for (int n = 0; n < S; ++n) out.A[(part * a.dim + d) * N + wave * S + n] = dA[n];
-        if (seg == 0 && a.grad_initial) {
+        if (block == 0 && a.grad_initial) {
 #pragma unroll
             for (int n = 0; n < S; ++n) a.grad_initial[((size_t)b * a.dim + d) * N + wave * S + n] = G[n];
         }
@@ -692,7 +739,7 @@ __global__ __launch_bounds__(1024) void scan_backward_sum_kernel(const rnntScan 
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const long long i = (long long)(blockIdx.x - bc_blocks) * kWave + lane;
     const long long rates = (long long)a.dim * N, columns = rates + 2 * a.dim;
-    const int parts = a.batch * g.segments, per = (parts + 15) / 16;
+    const int parts = a.batch * g.blocks, per = (parts + 15) / 16;
     const int p0 = wave * per, p1 = p0 + per < parts ? p0 + per : parts;
     float s = 0.f;
     if (i < columns) {
@@ -777,6 +824,7 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_forward_kernel(const r
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int d = (int)(blockIdx.x % groups) * kWave + lane;
     const long long item = (long long)(blockIdx.x / groups) * kConvWaves + wave;
+    const unsigned lo = d;
     const int run = (int)(item % runs);
     const long long b = item / runs;
     if (b >= c.batch || d >= c.dim) return;
@@ -787,8 +835,8 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_forward_kernel(const r
 #pragma unroll
     for (int k = 0; k < W; ++k) w[k] = c.weight[(size_t)d * W + k];
     const float bias = c.bias ? c.bias[d] : 0.f;
-    const E *x = static_cast<const E *>(c.x) + b * c.x_batch + d;
-    E *y = static_cast<E *>(c.y) + (size_t)b * c.length * c.dim + d;
+    const E *x = static_cast<const E *>(c.x) + b * c.x_batch;
+    E *y = static_cast<E *>(c.y) + (size_t)b * c.length * c.dim;
     if (te > t0) {
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) win[k + 1] = conv_in<DT, W>(c, (int)b, (long long)t0 - (W - 1) + k, d);
@@ -796,7 +844,7 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_forward_kernel(const r
     for (int tb = t0; tb < te; tb += kConvAhead) {
         E in[kConvAhead];
 #pragma unroll
-        for (int j = 0; j < kConvAhead; ++j) in[j] = x[(long long)(tb + j < te ? tb + j : te - 1) * c.x_time];
+        for (int j = 0; j < kConvAhead; ++j) in[j] = (x + (long long)(tb + j < te ? tb + j : te - 1) * c.x_time)[lo];
 #pragma unroll
         for (int j = 0; j < kConvAhead; ++j) {
             if (tb + j >= te) break;
@@ -806,10 +854,10 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_forward_kernel(const r
             float p = bias;
 #pragma unroll
             for (int k = 0; k < W; ++k) p = fma_(w[k], win[k], p);
-            y[(size_t)(tb + j) * c.dim] = DT::from_float(c.silu ? p * sigmoid_(p) : p);
+            (y + (size_t)(tb + j) * c.dim)[lo] = DT::from_float(c.silu ? p * sigmoid_(p) : p);
         }
     }
-    for (int t = te; t < t1; ++t) y[(size_t)t * c.dim] = DT::from_float(0.f);
+    for (int t = te; t < t1; ++t) (y + (size_t)t * c.dim)[lo] = DT::from_float(0.f);
     if (run == 0 && c.final_state) {
         float fin[W - 1];  // (all read before any is written: final_state may be the buffer of initial_state)
 #pragma unroll
@@ -832,6 +880,7 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_backward_kernel(const 
     const bool ok = d0 < c.dim;
     const int d = ok ? d0 : c.dim - 1;
     const long long item = (long long)(blockIdx.x / groups) * kConvWaves + wave;
+    const unsigned lo = d;
     const int run = (int)(item % runs);
     const long long b = item / runs;
     float dw[W], db = 0.f;
@@ -848,9 +897,9 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_backward_kernel(const 
             win[k] = 0.f;
         }
         const float bias = c.bias ? c.bias[d] : 0.f;
-        const E *x = static_cast<const E *>(c.x) + b * c.x_batch + d;
-        const E *gy = static_cast<const E *>(c.grad_y) + b * c.grad_y_batch + d;
-        E *dx = static_cast<E *>(c.grad_x) + (size_t)b * c.length * c.dim + d;
+        const E *x = static_cast<const E *>(c.x) + b * c.x_batch;
+        const E *gy = static_cast<const E *>(c.grad_y) + b * c.grad_y_batch;
+        E *dx = static_cast<E *>(c.grad_x) + (size_t)b * c.length * c.dim;
         E *di = c.grad_initial ? static_cast<E *>(c.grad_initial) + (size_t)b * (W - 1) * c.dim + d : nullptr;
         const E *gf = c.grad_final ? static_cast<const E *>(c.grad_final) + (size_t)b * (W - 1) * c.dim + d : nullptr;
         // Step s is newest in the window, gp[k] belongs to step s - (W - 1) + k; row t = s - (W - 1) of dx is then complete.
@@ -887,7 +936,7 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_backward_kernel(const 
             if (gf && t >= len - (W - 1) && t < len) v += DT::to_float(gf[(size_t)(t - (len - (W - 1))) * c.dim]);
             if (!ok) return;
             if (t >= 0)
-                dx[(size_t)t * c.dim] = DT::from_float(t < len ? v : 0.f);
+                (dx + (size_t)t * c.dim)[lo] = DT::from_float(t < len ? v : 0.f);
             else if (di)
                 di[(size_t)(t + W - 1) * c.dim] = DT::from_float(v);
         };
@@ -906,20 +955,20 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_backward_kernel(const 
                 E xin[kConvAhead], gin[kConvAhead];
 #pragma unroll
                 for (int j = 0; j < kConvAhead; ++j) {
-                    xin[j] = x[(long long)(s + j) * c.x_time];
-                    gin[j] = gy[(long long)(s + j) * c.grad_y_time];
+                    xin[j] = (x + (long long)(s + j) * c.x_time)[lo];
+                    gin[j] = (gy + (long long)(s + j) * c.grad_y_time)[lo];
                 }
 #pragma unroll
                 for (int j = 0; j < kConvAhead; ++j) {
                     step(s + j, DT::to_float(xin[j]), DT::to_float(gin[j]), true);
                     const float v = gradient();
-                    if (ok) dx[(size_t)(s + j - (W - 1)) * c.dim] = DT::from_float(v);
+                    if (ok) (dx + (size_t)(s + j - (W - 1)) * c.dim)[lo] = DT::from_float(v);
                 }
                 s += kConvAhead;
                 continue;
             }
             const bool live = s >= 0 && s < len;
-            step(s, s < len ? conv_in<DT, W>(c, (int)b, s, d) : 0.f, live ? DT::to_float(gy[(long long)s * c.grad_y_time]) : 0.f,
+            step(s, s < len ? conv_in<DT, W>(c, (int)b, s, d) : 0.f, live ? DT::to_float((gy + (long long)s * c.grad_y_time)[lo]) : 0.f,
                  live && s < t1);
             if (!live) gp[W - 1] = 0.f;  // (0 times an infinite derivative)
             if (s - (W - 1) >= first) finish(s - (W - 1));
@@ -1004,11 +1053,16 @@ inline ScanGeom scan_geometry(int batch, int length, int dim) {
     g.groups = groups_of(dim);
     g.padded = (length + kChunk - 1) / kChunk * kChunk;
     const long long waves = (long long)batch * g.groups;
-    long long want = waves >= 2048 ? 1 : (6144 + waves - 1) / waves;
+    const long long want = waves >= 2048 || length <= 64 ? 1 : (10240 + waves - 1) / waves;
     int len = (int)((length + want - 1) / want);
-    if (len < 64) len = 64;
+    const int least = waves * ((length + kChunk - 1) / kChunk) <= 2048 ? kChunk : 2 * kChunk;
+    if (len < least) len = least;
     g.seg_len = (len + kChunk - 1) / kChunk * kChunk;
     g.segments = (length + g.seg_len - 1) / g.seg_len;
+    const long long wgs = waves * g.segments;
+    g.joined = (int)(wgs > 4096 ? (wgs + 4095) / 4096 : 1);
+    if (g.joined > g.segments) g.joined = g.segments;
+    g.blocks = (g.segments + g.joined - 1) / g.joined;
     return g;
 }
 
@@ -1039,8 +1093,8 @@ inline ScanSpace scan_space(const ScanGeom &g, int batch, int length, int dim, i
     }
     if (backward) {
         s.BC = take((size_t)batch * length * g.groups * 2 * state);
-        s.A = take((size_t)batch * g.segments * dim * state);
-        s.D = take((size_t)batch * g.segments * 2 * dim);
+        s.A = take((size_t)batch * g.blocks * dim * state);
+        s.D = take((size_t)batch * g.blocks * 2 * dim);
     }
     s.total = at;
     return s;
@@ -1053,8 +1107,11 @@ inline bool scan_args_ok(const rnntScan *a) {
 template <int N, bool BACKWARD>
 void launch_join(const rnntScan &a, const ScanGeom &g, hipStream_t st) {
     const long long n = (long long)a.batch * a.dim * (N / 4);
-    hipLaunchKernelGGL((scan_join_kernel<N, BACKWARD>), dim3((unsigned)((n + kWave - 1) / kWave)), dim3(kJoinWaves * kWave), 0, st, a,
-                       g);
+    const dim3 grid((unsigned)((n + kWave - 1) / kWave));
+    if (g.segments <= kJoinAhead)
+        hipLaunchKernelGGL((scan_join_kernel<N, BACKWARD, 1>), grid, dim3(kWave), 0, st, a, g);
+    else
+        hipLaunchKernelGGL((scan_join_kernel<N, BACKWARD, kJoinWaves>), grid, dim3(kJoinWaves * kWave), 0, st, a, g);
 }
 
 template <typename DT, int N>
@@ -1091,7 +1148,7 @@ rnntStatus_t scan_backward(const rnntScan &a, hipStream_t st) {
     }
     const ScanPartials p = {reinterpret_cast<float *>(ws + s.BC), reinterpret_cast<float *>(ws + s.A),
                             reinterpret_cast<float *>(ws + s.D)};
-    hipLaunchKernelGGL((scan_backward_kernel<DT, N>), dim3(grid), dim3(N * 16), 0, st, a, g, p);
+    hipLaunchKernelGGL((scan_backward_kernel<DT, N>), dim3((unsigned)((long long)a.batch * g.blocks * g.groups)), dim3(N * 16), 0, st, a, g, p);
     const unsigned bc = (unsigned)(((long long)a.batch * a.length * 2 * N + 1023) / 1024);
     const unsigned pa = (unsigned)(((long long)a.dim * (N + 2) + kWave - 1) / kWave);
     hipLaunchKernelGGL((scan_backward_sum_kernel<DT, N>), dim3(bc + pa), dim3(1024), 0, st, a, g, p, bc);
