@@ -396,7 +396,8 @@ rnntStatus_t rnnt_row_max_logp(const void *x, int rows, int V, rnntDtype_t dtype
  * rnnt_row_rules writes out / logp (logp may be NULL) as rnnt_row_max_logp does: a row that its mask empties gives
  * token 0 and a NaN score, as a row of -inf there.  rnnt_process_logits writes x' itself, rounded to the logits' type
  * once; processed may be x (in place).
- * history_stride <= RNNT_MAX_HISTORY (the counters hold 16 bits).
+ * history_stride <= RNNT_MAX_HISTORY (the counters hold 16 bits).  workspace: rnnt_row_rules_workspace_size bytes (0 for
+ * rows of ordinary length: NULL then), 16-byte aligned.  V <= 2^30.
  */
 #define RNNT_MAX_HISTORY 65535
 typedef struct {
@@ -410,8 +411,9 @@ typedef struct {
     long long allowed_stride;
     float repetition_penalty, presence_penalty, frequency_penalty;
 } rnntRules;
+rnntStatus_t rnnt_row_rules_workspace_size(int rows, int V, rnntDtype_t dtype, size_t *size_bytes);
 rnntStatus_t rnnt_row_rules(const void *x, int rows, int V, rnntDtype_t dtype, const rnntRules *rules, int *out,
-                            float *logp, void *stream);
+                            float *logp, void *workspace, void *stream);
 rnntStatus_t rnnt_process_logits(const void *x, int rows, int V, rnntDtype_t dtype, const rnntRules *rules,
                                  void *processed, void *stream);
 

@@ -58,6 +58,7 @@ EXPORTED_SYMBOLS = (
     "rnnt_joint_hidden_backward_compact",
     "rnnt_row_argmax",
     "rnnt_row_max_logp",
+    "rnnt_row_rules_workspace_size",
     "rnnt_row_rules",
     "rnnt_process_logits",
     "rnnt_token_embedding_forward",
@@ -248,7 +249,8 @@ def load() -> ctypes.CDLL:
         lib.rnnt_row_argmax.restype = ctypes.c_int
         lib.rnnt_row_max_logp.argtypes = [vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, vp, vp, ctypes.c_void_p]
         lib.rnnt_row_max_logp.restype = ctypes.c_int
-        lib.rnnt_row_rules.argtypes = [vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.POINTER(RnntRules), vp, vp, vp]
+        lib.rnnt_row_rules.argtypes = [vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.POINTER(RnntRules), vp, vp, vp, vp]
+        lib.rnnt_row_rules_workspace_size.argtypes = [ctypes.c_int] * 3 + [ctypes.POINTER(ctypes.c_size_t)]
         lib.rnnt_process_logits.argtypes = [vp, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.POINTER(RnntRules), vp, vp]
         lib.rnnt_token_embedding_forward.argtypes = [vp, ctypes.c_int, ctypes.c_longlong, vp, ctypes.c_longlong, ctypes.c_int,
                                                      ctypes.c_int, ctypes.c_float, ctypes.c_int, vp, vp]

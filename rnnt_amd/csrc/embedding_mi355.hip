@@ -23,7 +23,7 @@ constexpr int kBatch = 8;         // gradient rows loaded at once
 constexpr int kRankMax = 4096;    // up to this many positions are sorted by counting smaller ones
 constexpr int kRankRows = 64;     // rows of the gradient that a workgroup of the counting kernel clears
 constexpr int kSortItems = 1024;  // positions per workgroup and pass of the radix sort
-constexpr int kJoinWaves = 8;
+constexpr int kJoinWaves = 8, kJoinAlone = 64;
 constexpr int kDigits = 256;
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -185,6 +185,7 @@ __global__ __launch_bounds__(kBlock) void embed_place_kernel(const void *__restr
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const long long base = (long long)blockIdx.x * kSortItems + wave * (kSortItems / kWaves);
     int before = 0, total = 0;  // of digit threadIdx.x: in the workgroups before this one, in all
+#pragma unroll 16
     for (int w = 0; w < (int)gridDim.x; ++w) {
         const int c = counts[(size_t)w * kDigits + threadIdx.x];
         before += w < (int)blockIdx.x ? c : 0;
@@ -327,50 +328,80 @@ __global__ __launch_bounds__(kBlock) void embed_sum_kernel(const int *__restrict
     close(cur == next);
 }
 
-// The runs that cross pieces: the workgroup of the piece a run begins in adds the run's parts, each wave a range of
-// the pieces in order, then the waves' sums in order.  grid.y: slices of 64 VEC columns.
+// The runs that cross pieces, joined by the wave of the piece a run begins in, in order; a run of more than kJoinAlone
+// pieces (a token that is a tenth of all positions) by the whole workgroup, each wave a range of its pieces in order, then
+// the waves' sums in order.  grid.y: slices of 64 VEC columns.
 template <typename DT, int VEC>
 __global__ __launch_bounds__(kJoinWaves *kWave) void embed_join_kernel(const int *__restrict__ sorted, int n, int vocab, int dim,
                                                                        float scale, typename DT::elem *__restrict__ grad_weight,
-                                                                       const float *__restrict__ partial, int piece) {
+                                                                       const float *__restrict__ partial, int piece, int pieces) {
     __shared__ float s_acc[kJoinWaves][kWave * VEC];
-    const int p = blockIdx.x;
-    const int begin = p * piece, end = begin + piece;
-    if (end >= n) return;
-    const int tok = sorted[end - 1];
-    if (tok == vocab || sorted[end] != tok) return;
-    if (sorted[begin] == tok && begin > 0 && sorted[begin - 1] == tok) return;  // began earlier
-    const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-    const int stop = lower_bound(sorted, n, tok + 1);  // end of the run
-    const int last = (stop - 1) / piece;               // pieces p + 1 .. last hold parts of it
-    const int parts = last - p, per = (parts + kJoinWaves - 1) / kJoinWaves;
-    const int p0 = p + 1 + wave * per, p1 = p0 + per < last + 1 ? p0 + per : last + 1;
+    __shared__ int s_last[kJoinWaves], s_tok[kJoinWaves];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int p = blockIdx.x * kJoinWaves + wave, begin = p * piece, end = begin + piece;
     const int c = (int)blockIdx.y * kWave * VEC + lane * VEC;
-    float acc[VEC] = {};
-    if (c < dim) {
-        if (wave == 0) {
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[j] = partial[((size_t)p * 2 + 1) * dim + c + j];
-        }
+    auto add_parts = [&](int p0, int p1, float (&acc)[VEC]) {  // the parts [p0, p1) of a run that began earlier
 #pragma unroll 8
         for (int q = p0; q < p1; ++q) {
 #pragma unroll
             for (int j = 0; j < VEC; ++j) acc[j] += partial[(size_t)q * 2 * dim + c + j];
         }
-    }
+    };
+    auto first_part = [&](int q, float (&acc)[VEC]) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) s_acc[wave][lane * VEC + j] = acc[j];
+        for (int j = 0; j < VEC; ++j) acc[j] = partial[((size_t)q * 2 + 1) * dim + c + j];
+    };
+    int last = -1, tok = vocab;  // pieces p + 1 .. last hold parts of the run that begins in piece p and goes on
+    if (p < pieces && end < n) {
+        tok = sorted[end - 1];
+        const bool goes_on = tok != vocab && sorted[end] == tok;
+        if (goes_on && !(sorted[begin] == tok && begin > 0 && sorted[begin - 1] == tok)) {
+            last = p + 1;
+            while (last < p + 4 && (last + 1) * (long long)piece < n && sorted[(last + 1) * piece] == tok) ++last;
+            if (last == p + 4) last = (lower_bound(sorted, n, tok + 1) - 1) / piece;
+        }
+    }
+    const bool alone = last >= 0 && last - p <= kJoinAlone;
+    if (alone && c < dim) {
+        float acc[VEC];
+        first_part(p, acc);
+        add_parts(p + 1, last + 1, acc);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] *= scale;
+        store_piece<DT, VEC>(grad_weight + (size_t)tok * dim + c, acc);
+    }
+    if (lane == 0) {
+        s_last[wave] = alone ? -1 : last;
+        s_tok[wave] = tok;
+    }
     __syncthreads();
-    if (wave != 0 || c >= dim) return;
-    float f[VEC];
+    for (int w = 0; w < kJoinWaves; ++w) {
+        if (s_last[w] < 0) continue;  // (the same for the whole workgroup)
+        const int from = blockIdx.x * kJoinWaves + w, to = s_last[w];
+        const int per = (to - from + kJoinWaves - 1) / kJoinWaves;
+        const int p0 = from + 1 + wave * per, p1 = p0 + per < to + 1 ? p0 + per : to + 1;
+        float acc[VEC] = {};
+        if (c < dim) {
+            if (wave == 0) first_part(from, acc);
+            add_parts(p0, p1, acc);
+        }
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        float s = 0.f;
+        for (int j = 0; j < VEC; ++j) s_acc[wave][lane * VEC + j] = acc[j];
+        __syncthreads();
+        if (wave == 0 && c < dim) {
+            float f[VEC];
 #pragma unroll
-        for (int w = 0; w < kJoinWaves; ++w) s += s_acc[w][lane * VEC + j];
-        f[j] = s * scale;
+            for (int j = 0; j < VEC; ++j) {
+                float s = 0.f;
+#pragma unroll
+                for (int q = 0; q < kJoinWaves; ++q) s += s_acc[q][lane * VEC + j];
+                f[j] = s * scale;
+            }
+            store_piece<DT, VEC>(grad_weight + (size_t)s_tok[w] * dim + c, f);
+        }
+        __syncthreads();
     }
-    store_piece<DT, VEC>(grad_weight + (size_t)tok * dim + c, f);
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------------
@@ -473,9 +504,9 @@ rnntStatus_t embed_backward_with(const void *tokens, int tokens_64, int n, const
                        static_cast<const int *>(sorted[at]), static_cast<const int *>(order[at]), n, grad, grad_stride, vocab, dim, scale,
                        grad_weight, partial, piece, pieces, slices, shift, (unsigned)blocks);
     if (pieces > 1)
-        hipLaunchKernelGGL((embed_join_kernel<DT, VEC>), dim3((unsigned)pieces, (unsigned)((dim + kWave * VEC - 1) / (kWave * VEC))),
+        hipLaunchKernelGGL((embed_join_kernel<DT, VEC>), dim3((unsigned)((pieces + kJoinWaves - 1) / kJoinWaves), (unsigned)((dim + kWave * VEC - 1) / (kWave * VEC))),
                            dim3(kJoinWaves * kWave), 0, st, static_cast<const int *>(sorted[at]), n, vocab, dim, scale, grad_weight,
-                           static_cast<const float *>(partial), piece);
+                           static_cast<const float *>(partial), piece, pieces);
     return hipGetLastError() == hipSuccess ? RNNT_STATUS_SUCCESS : RNNT_STATUS_EXECUTION_FAILED;
 }
 

@@ -500,7 +500,8 @@ RulesIn rules_check(const Tensor &x, const MaybeTensor &bias_in, const MaybeTens
     TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) >= 1 && x.size(1) >= 1, "x must be a non-empty [rows, V] tensor");
     dtype_code(x, "x");
     in.rows = as_int(x.size(0), "rows");
-    in.V = as_int(x.size(1), "V");
+    TORCH_CHECK_VALUE(x.size(1) <= (1 << 30), "V is too large");
+    in.V = (int)x.size(1);
     int64_t contexts = 1;
     const char *by = nullptr;
     auto agree = [&](const Tensor &t, const char *name) {
@@ -568,8 +569,11 @@ std::tuple<Tensor, Tensor> row_rules_op(const Tensor &x, const MaybeTensor &bias
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     Tensor token = at::empty({in.rows}, x.options().dtype(at::kInt));
     Tensor logp = at::empty({want_logp ? in.rows : 0}, x.options().dtype(at::kFloat));
+    size_t need = 0;
+    check_status(rnnt_row_rules_workspace_size(in.rows, in.V, dtype_code(x, "x"), &need), "rnnt_row_rules_workspace_size");
+    const Tensor ws = need ? bytes(need, x) : Tensor();
     check_status(rnnt_row_rules(in.x.data_ptr(), in.rows, in.V, dtype_code(x, "x"), &in.r, pointer<int>(token),
-                                want_logp ? pointer<float>(logp) : nullptr, stream_of(x)),
+                                want_logp ? pointer<float>(logp) : nullptr, pointer<void>(ws), stream_of(x)),
                  "rnnt_row_rules");
     return {token, logp};
 }

@@ -215,9 +215,14 @@ def test_c_entry_points_refuse_before_any_launch():
     assert lib.rnnt_token_embedding_backward(one, 0, 3, one, 4, 5, 4, 1.0, -1, 0, one, None, None) == 2
     assert lib.rnnt_token_embedding_backward(one, 0, 3, one, 4, 5, 4, 1.0, -1, 0, one, ctypes.c_void_p(8), None) == 2
 
-    assert lib.rnnt_row_rules(one, 4, 8, 0, None, one, None, None) == 2
+    assert lib.rnnt_row_rules(one, 4, 8, 0, None, one, None, None, None) == 2
     rules = _lib.RnntRules(contexts=3, repetition_penalty=1.0)
-    assert lib.rnnt_row_rules(one, 4, 8, 0, ctypes.byref(rules), one, None, None) == 2             # 4 rows of 3 contexts
+    assert lib.rnnt_row_rules(one, 4, 8, 0, ctypes.byref(rules), one, None, None, None) == 2             # 4 rows of 3 contexts
+    rules = _lib.RnntRules(contexts=1, repetition_penalty=1.0)
+    assert lib.rnnt_row_rules(one, 4, 70001, 0, ctypes.byref(rules), one, None, None, None) == 2   # needs its workspace
+    assert lib.rnnt_row_rules_workspace_size(4, 5455, 1, ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.rnnt_row_rules_workspace_size(4, 70001, 1, ctypes.byref(n)) == 0 and n.value > 0
+    assert lib.rnnt_row_rules_workspace_size(4, 70001, 3, ctypes.byref(n)) == 2
     for change in (dict(history=16, history_stride=0), dict(history=16, history_stride=65536), dict(bias=16, bias_stride=7),
                    dict(allowed=16, allowed_stride=0, repetition_penalty=0.0), dict(repetition_penalty=float("nan")),
                    dict(presence_penalty=float("nan")), dict(contexts=0)):
