@@ -426,7 +426,8 @@ rnntStatus_t rnnt_process_logits(const void *x, int rows, int V, rnntDtype_t dty
  * row of NaN.  backward: grad_weight[v, :] = scale * (sum of grad_out[i, :] over the positions i with tokens[i] = v, in
  * position order, fp32), rounded once, for EVERY v in [0, vocab): zeros where no position holds v, and for
  * v = padding_idx (-1: none); tokens outside [0, vocab) add nothing.  grad_out rows are grad_stride elements apart.  No
- * atomics.  workspace: rnnt_token_embedding_workspace_size bytes, 16-byte aligned.  n < 2^31 - 2^16.
+ * atomics.  workspace: rnnt_token_embedding_workspace_size bytes, 16-byte aligned (0 for short sequences: NULL then).
+ * n < 2^31 - 2^16.
  */
 rnntStatus_t rnnt_token_embedding_forward(const void *tokens, int tokens_64, long long n, const void *weight,
                                           long long weight_stride, int vocab, int dim, float scale, rnntDtype_t dtype,

@@ -20,6 +20,8 @@ using namespace rnnt_mi355_detail;
 
 constexpr int kBlock = 256;
 constexpr int kBatch = 8;         // gradient rows loaded at once
+constexpr int kListMax = 2048;    // up to this many positions are not sorted: every workgroup lists its own rows' positions
+constexpr int kListRows = 16, kListWaves = 8, kListAlone = 64;
 constexpr int kRankMax = 4096;    // up to this many positions are sorted by counting smaller ones
 constexpr int kRankRows = 64;     // rows of the gradient that a workgroup of the counting kernel clears
 constexpr int kSortItems = 1024;  // positions per workgroup and pass of the radix sort
@@ -404,6 +406,130 @@ __global__ __launch_bounds__(kJoinWaves *kWave) void embed_join_kernel(const int
     }
 }
 
+// Few positions and few to a token: one launch, no sorting.  A workgroup has 16 rows of the gradient: it goes through all
+// tokens, lists in LDS the positions of its rows (each wave an eighth of the positions, so that the list is in order),
+// and sums them, a wave to a row; a row of more than kListAlone positions is shared by the waves, a range each, and their
+// sums are added in order.
+template <typename DT, int VEC>
+__global__ __launch_bounds__(kListWaves *kWave) void embed_list_kernel(const void *__restrict__ tokens, int tokens_64, int n, int vocab,
+                                                                       long long padding, const typename DT::elem *__restrict__ grad,
+                                                                       long long grad_stride, int dim, float scale,
+                                                                       typename DT::elem *__restrict__ grad_weight) {
+    constexpr int kPart = kListMax / kListWaves;
+    __shared__ int s_found[kListWaves][kPart], s_count[kListWaves], s_list[kListMax];
+    __shared__ int s_many[kListRows];
+    __shared__ float s_acc[kListWaves][kWave * VEC];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int v0 = blockIdx.x * kListRows;
+    const int c = (int)blockIdx.y * kWave * VEC + lane * VEC;
+    {
+        const int per = (n + kListWaves - 1) / kListWaves, i0 = wave * per, i1 = i0 + per < n ? i0 + per : n;
+        int count = 0, key[kPart / kWave];
+#pragma unroll
+        for (int u = 0; u < kPart / kWave; ++u) {
+            const int i = i0 + u * kWave + lane;
+            key[u] = i < i1 ? key_at(tokens, tokens_64, i, vocab, padding) : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < kPart / kWave; ++u) {
+            const int i = i0 + u * kWave + lane, k = key[u] < 0 ? -1 : key[u] - v0;
+            const bool mine = k >= 0 && k < kListRows && v0 + k < vocab;  // (the key of a position without a row is vocab)
+            const unsigned long long found = __ballot(mine);
+            if (mine) s_found[wave][count + __popcll(found & ((1ull << lane) - 1))] = i * kListRows + k;
+            count += __popcll(found);
+        }
+        if (lane == 0) s_count[wave] = count;
+        if (threadIdx.x < kListRows) s_many[threadIdx.x] = 0;
+    }
+    __syncthreads();
+    int total = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < kListWaves; ++w) {
+        const int k = s_count[w];
+        before += w < wave ? k : 0;
+        total += k;
+    }
+    for (int k = lane; k < s_count[wave]; k += kWave) s_list[before + k] = s_found[wave][k];
+    __syncthreads();
+
+    auto matches = [&](int r, int b, int &entry) {
+        entry = b + lane < total ? s_list[b + lane] : -1;
+        return __ballot(entry >= 0 && entry % kListRows == r);
+    };
+    // the sum of row r's positions [from, to) in order
+    auto sum = [&](int r, int from, int to, float (&acc)[VEC]) {
+        int seen = 0;
+        for (int b = 0; b < total && seen < to; b += kWave) {
+            int entry;
+            unsigned long long found = matches(r, b, entry);
+            const int here = __popcll(found);
+            if (seen + here > from) {
+                for (int skip = seen; skip < from; ++skip) found &= found - 1;
+                int left = (seen + here < to ? seen + here : to) - (seen > from ? seen : from);
+                while (left > 0) {
+                    float f[kBatch][VEC];
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+                        if (k < left) {
+                            const int at = __builtin_amdgcn_readlane(entry, __builtin_ctzll(found)) / kListRows;
+                            found &= found - 1;
+                            if (c < dim) load_piece<DT, VEC>(grad + (size_t)at * grad_stride + c, f[k]);
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) {
+                        if (k < left) {
+#pragma unroll
+                            for (int j = 0; j < VEC; ++j) acc[j] += f[k][j];
+                        }
+                    }
+                    left -= kBatch;
+                }
+            }
+            seen += here;
+        }
+    };
+    auto store = [&](int r, float (&acc)[VEC]) {
+        if (c >= dim) return;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] *= scale;
+        store_piece<DT, VEC>(grad_weight + (size_t)(v0 + r) * dim + c, acc);
+    };
+    for (int r = wave; r < kListRows && v0 + r < vocab; r += kListWaves) {
+        int many = 0, entry;
+        for (int b = 0; b < total; b += kWave) many += __popcll(matches(r, b, entry));
+        if (many > kListAlone) {
+            if (lane == 0) s_many[r] = many;
+            continue;
+        }
+        float acc[VEC] = {};
+        sum(r, 0, many, acc);
+        store(r, acc);
+    }
+    __syncthreads();
+    for (int r = 0; r < kListRows; ++r) {
+        const int many = s_many[r];
+        if (many == 0) continue;  // (the same for the whole workgroup)
+        const int per = (many + kListWaves - 1) / kListWaves, from = wave * per, to = from + per < many ? from + per : many;
+        float acc[VEC] = {};
+        if (from < to) sum(r, from, to, acc);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s_acc[wave][lane * VEC + j] = acc[j];
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                acc[j] = 0.f;
+#pragma unroll
+                for (int w = 0; w < kListWaves; ++w) acc[j] += s_acc[w][lane * VEC + j];
+            }
+            store(r, acc);
+        }
+        __syncthreads();
+    }
+}
+
 // ---- host side ---------------------------------------------------------------------------------------------------------
 struct EmbedSpace {
     size_t sorted[2], order[2], counts, partial, total;
@@ -416,7 +542,9 @@ inline int piece_of(long long n) {
 }
 inline int pieces_of(long long n) { return (int)((n + piece_of(n) - 1) / piece_of(n)); }
 inline int sort_blocks(long long n) { return (int)((n + kSortItems - 1) / kSortItems); }
-inline EmbedSpace embed_space(long long n, int dim) {
+// At most 16 positions to a row on average: a workgroup's 16 rows then have few enough to be summed by its waves.
+inline bool listed(long long n, int vocab) { return n <= kListMax && n <= 16ll * vocab; }
+inline EmbedSpace embed_space(long long n, int vocab, int dim) {
     EmbedSpace s = {};
     size_t at = 0;
     auto take = [&at](size_t bytes) {
@@ -424,6 +552,7 @@ inline EmbedSpace embed_space(long long n, int dim) {
         at += (bytes + 15) & ~(size_t)15;
         return here;
     };
+    if (listed(n, vocab)) return s;
     const int copies = n > kRankMax ? 2 : 1;
     for (int i = 0; i < copies; ++i) {
         s.sorted[i] = take((size_t)n * 4);
@@ -467,7 +596,14 @@ template <typename DT, int VEC>
 rnntStatus_t embed_backward_with(const void *tokens, int tokens_64, int n, const typename DT::elem *grad, long long grad_stride,
                                  int vocab, int dim, float scale, long long padding, typename DT::elem *grad_weight, void *workspace,
                                  hipStream_t st) {
-    const EmbedSpace sp = embed_space(n, dim);
+    if (listed(n, vocab)) {
+        hipLaunchKernelGGL((embed_list_kernel<DT, VEC>),
+                           dim3((unsigned)((vocab - 1) / kListRows + 1), (unsigned)((dim + kWave * VEC - 1) / (kWave * VEC))),
+                           dim3(kListWaves * kWave), 0, st, tokens, tokens_64, n, vocab, padding, grad, grad_stride, dim, scale,
+                           grad_weight);
+        return hipGetLastError() == hipSuccess ? RNNT_STATUS_SUCCESS : RNNT_STATUS_EXECUTION_FAILED;
+    }
+    const EmbedSpace sp = embed_space(n, vocab, dim);
     char *ws = static_cast<char *>(workspace);
     int *sorted[2], *order[2];
     for (int i = 0; i < 2; ++i) {
@@ -540,15 +676,15 @@ rnntStatus_t rnnt_token_embedding_forward(const void *tokens, int tokens_64, lon
 
 rnntStatus_t rnnt_token_embedding_workspace_size(long long n, int vocab, int dim, size_t *size_bytes) {
     if (size_bytes == nullptr || !embed_shape_ok(n, vocab, dim)) return RNNT_STATUS_INVALID_VALUE;
-    *size_bytes = embed_space(n, dim).total;
+    *size_bytes = embed_space(n, vocab, dim).total;
     return RNNT_STATUS_SUCCESS;
 }
 
 rnntStatus_t rnnt_token_embedding_backward(const void *tokens, int tokens_64, long long n, const void *grad_out,
                                            long long grad_stride, int vocab, int dim, float scale, long long padding_idx,
                                            rnntDtype_t dtype, void *grad_weight, void *workspace, void *stream) {
-    if (tokens == nullptr || grad_out == nullptr || grad_weight == nullptr || workspace == nullptr || !aligned16(workspace) ||
-        !embed_shape_ok(n, vocab, dim) || grad_stride < 0)
+    if (tokens == nullptr || grad_out == nullptr || grad_weight == nullptr || !embed_shape_ok(n, vocab, dim) || grad_stride < 0 ||
+        (embed_space(n, vocab, dim).total > 0 && (workspace == nullptr || !aligned16(workspace))))
         return RNNT_STATUS_INVALID_VALUE;
     hipStream_t st = static_cast<hipStream_t>(stream);
     switch (dtype) {

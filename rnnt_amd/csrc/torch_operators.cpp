@@ -125,11 +125,11 @@ public:
         Tensor dweight = at::empty({vocab, dim}, g.options());
         size_t need = 0;
         check_status(rnnt_token_embedding_workspace_size(n, (int)vocab, (int)dim, &need), "rnnt_token_embedding_workspace_size");
-        const Tensor ws = bytes(need, g);
+        const Tensor ws = need ? bytes(need, g) : Tensor();
         check_status(rnnt_token_embedding_backward(tokens.data_ptr(), tokens.scalar_type() == at::kLong, n, g.data_ptr(), g.stride(0),
                                                    (int)vocab, (int)dim, (float)ctx->saved_data["scale"].toDouble(),
                                                    ctx->saved_data["padding"].toInt(), dtype_code(g, "grad"), dweight.data_ptr(),
-                                                   ws.data_ptr(), stream_of(g)),
+                                                   pointer<void>(ws), stream_of(g)),
                      "rnnt_token_embedding_backward");
         return once({Tensor(), dweight, Tensor(), Tensor()}, "token_embedding");
     }

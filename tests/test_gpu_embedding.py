@@ -63,6 +63,19 @@ def test_one_token_everywhere_and_no_token_of_a_row():
         assert torch.count_nonzero(dw[:49]) == 0
 
 
+@pytest.mark.parametrize("n,V", [(2048, 128), (2048, 127), (2049, 4000), (700, 50), (129, 1000)])
+def test_frequent_tokens_in_short_sequences(n, V):
+    """Both sides of the rule that picks the unsorted kernel (2048 positions, 16 to a row), with one row of most of them and
+    two of more than a wave sums alone."""
+    tokens, weight, grad = make(n, V, 72, torch.float32, seed=n)
+    tokens[: n // 2] = V - 1
+    tokens[n // 2::3] = 0
+    check(tokens, weight, grad, 1.25, None)
+    check(tokens, weight.bfloat16(), grad.bfloat16(), 1.25, 0)
+    wide, more = torch.randn(V, 600, generator=torch.Generator().manual_seed(1)), torch.randn(n, 600, generator=torch.Generator().manual_seed(2))
+    check(tokens, wide, more, 1.0, None)
+
+
 def test_layouts():
     """Rows of the weight and of the gradient that lie apart, start off 16 bytes, repeat, or belong to a broadcast gradient."""
     tokens, weight, grad = make(90, 20, 24, torch.float16, seed=8)

@@ -211,9 +211,11 @@ def test_c_entry_points_refuse_before_any_launch():
     assert lib.rnnt_token_embedding_forward(one, 0, 3, one, 4, 5, 4, 1.0, 7, one, None) == 2       # no such type
     assert lib.rnnt_token_embedding_workspace_size(0, 5, 4, ctypes.byref(n)) == 2
     assert lib.rnnt_token_embedding_workspace_size(3, 5, 4, None) == 2
-    assert lib.rnnt_token_embedding_workspace_size(3, 5, 4, ctypes.byref(n)) == 0 and n.value > 0
-    assert lib.rnnt_token_embedding_backward(one, 0, 3, one, 4, 5, 4, 1.0, -1, 0, one, None, None) == 2
-    assert lib.rnnt_token_embedding_backward(one, 0, 3, one, 4, 5, 4, 1.0, -1, 0, one, ctypes.c_void_p(8), None) == 2
+    assert lib.rnnt_token_embedding_workspace_size(3, 5, 4, ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.rnnt_token_embedding_workspace_size(3000, 5, 4, ctypes.byref(n)) == 0 and n.value > 0
+    assert lib.rnnt_token_embedding_backward(one, 0, 3, one, 4, 5, 4, 1.0, -1, 0, None, None, None) == 2
+    assert lib.rnnt_token_embedding_backward(one, 0, 3000, one, 4, 5, 4, 1.0, -1, 0, one, None, None) == 2
+    assert lib.rnnt_token_embedding_backward(one, 0, 3000, one, 4, 5, 4, 1.0, -1, 0, one, ctypes.c_void_p(8), None) == 2
 
     assert lib.rnnt_row_rules(one, 4, 8, 0, None, one, None, None, None) == 2
     rules = _lib.RnntRules(contexts=3, repetition_penalty=1.0)
