@@ -843,8 +843,12 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_forward_kernel(const r
     }
     for (int tb = t0; tb < te; tb += kConvAhead) {
         E in[kConvAhead];
+        const E *px = x + (long long)tb * c.x_time;
 #pragma unroll
-        for (int j = 0; j < kConvAhead; ++j) in[j] = (x + (long long)(tb + j < te ? tb + j : te - 1) * c.x_time)[lo];
+        for (int j = 0; j < kConvAhead; ++j) {
+            in[j] = px[lo];
+            if (tb + j + 1 < te) px += c.x_time;
+        }
 #pragma unroll
         for (int j = 0; j < kConvAhead; ++j) {
             if (tb + j >= te) break;
@@ -950,19 +954,29 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_backward_kernel(const 
         int s = first;
         const int stop = t1 + W - 1;
         while (s < stop) {
-            // whole blocks inside the sequence and the run, whose dx rows are ordinary ones: loads first, no tests
-            if (s >= W - 1 && s - (W - 1) >= first && s + kConvAhead <= t1 && s + kConvAhead <= len - (W - 1)) {
+            // whole blocks of the sequence and the run (no part of the final state: t < len - (W - 1)): loads first, no tests
+            if (s >= 0 && s + kConvAhead <= t1 && s + kConvAhead <= len) {
                 E xin[kConvAhead], gin[kConvAhead];
+                const E *px = x + (long long)s * c.x_time, *pg = gy + (long long)s * c.grad_y_time;
 #pragma unroll
                 for (int j = 0; j < kConvAhead; ++j) {
-                    xin[j] = (x + (long long)(s + j) * c.x_time)[lo];
-                    gin[j] = (gy + (long long)(s + j) * c.grad_y_time)[lo];
+                    xin[j] = px[lo];
+                    gin[j] = pg[lo];
+                    px += c.x_time;
+                    pg += c.grad_y_time;
                 }
+                const int t = s - (W - 1);
+                E *pd = dx + (long long)t * c.dim;
 #pragma unroll
                 for (int j = 0; j < kConvAhead; ++j) {
                     step(s + j, DT::to_float(xin[j]), DT::to_float(gin[j]), true);
                     const float v = gradient();
-                    if (ok) (dx + (size_t)(s + j - (W - 1)) * c.dim)[lo] = DT::from_float(v);
+                    if (j >= W - 1 || t + j >= t0) {
+                        if (ok) pd[lo] = DT::from_float(v);
+                    } else if (t + j < 0 && di && ok) {
+                        di[(size_t)(t + j + W - 1) * c.dim] = DT::from_float(v);
+                    }
+                    pd += c.dim;
                 }
                 s += kConvAhead;
                 continue;
