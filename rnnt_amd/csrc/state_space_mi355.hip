@@ -306,9 +306,14 @@ __global__ __launch_bounds__(WAVES *kWave) void scan_join_kernel(const rnntScan 
     const bool ok = b < a.batch;
     const int per = (g.segments + WAVES - 1) / WAVES;
     const int k0 = wave * per, k1 = !ok ? k0 : (k0 + per < g.segments ? k0 + per : g.segments);
-    float A2[4], h[4] = {0.f, 0.f, 0.f, 0.f};
+    float A2[4] = {}, h[4] = {}, start[4] = {};
+    const float *from = BACKWARD ? a.grad_final : a.initial_state;
+    if (ok) {
+        load_row<4>(a.A + (size_t)d * N + q * 4, A2);
+        if (from) load_row<4>(from + ((size_t)b * a.dim + d) * N + q * 4, start);
+    }
 #pragma unroll
-    for (int n = 0; n < 4; ++n) A2[n] = ok ? a.A[(size_t)d * N + q * 4 + n] * kLog2e : 0.f;
+    for (int n = 0; n < 4; ++n) A2[n] *= kLog2e;
     f32x4 *tiles = reinterpret_cast<f32x4 *>(g.seg_state) + ((size_t)b * g.segments * (N / 4) + q) * a.dim + d;
     const float *deltas = g.seg_delta + (size_t)b * g.segments * a.dim + d;
     auto walk = [&](bool write) {
@@ -340,10 +345,9 @@ __global__ __launch_bounds__(WAVES *kWave) void scan_join_kernel(const rnntScan 
         for (int n = 0; n < 4; ++n) s_end[wave][n][lane] = h[n];
         __syncthreads();
     }
-    const float *from = BACKWARD ? a.grad_final : a.initial_state;
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-        h[n] = from && ok ? from[((size_t)b * a.dim + d) * N + q * 4 + n] : 0.f;
+        h[n] = start[n];
         for (int w = 0; w < wave; ++w) h[n] = fma_(exp2_(s_delta[w][lane] * A2[n]), h[n], s_end[w][n][lane]);
     }
     walk(true);
@@ -508,6 +512,7 @@ template <typename DT, int N>
 __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan a, const ScanGeom g, const ScanPartials out) {
     typedef typename DT::elem E;
     constexpr int S = 4, W = N / S, kMine = kChunk / W;
+    constexpr int kShare = kChunk * 2 * N / (W * kWave);  // values of a chunk's rows, and of its dB and dC, per thread
     __shared__ float s_delta[kChunk][kWave], s_x[kChunk][kWave], s_gy[kChunk][kWave];
     __shared__ float s_part[3][W][kChunk][kWave];
     __shared__ float s_bc[kChunk][2 * N];
@@ -553,7 +558,7 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
     const E *zp = gated ? static_cast<const E *>(a.z) + b * a.z_batch : xp;
     const long long z_time = gated ? a.z_time : a.x_time;
     const E *gp = static_cast<const E *>(a.grad_y) + b * a.grad_y_batch;
-    const f32x2 *rows = reinterpret_cast<const f32x2 *>(g.rows + (size_t)b * g.padded * 2 * N) + threadIdx.x;
+    const float *rows = g.rows + (size_t)b * g.padded * 2 * N + threadIdx.x;
     const size_t out0 = (size_t)b * a.length * a.dim;
     E *dxp = static_cast<E *>(a.grad_x) + out0, *ddtp = static_cast<E *>(a.grad_dt) + out0;
     E *dzp = gated ? static_cast<E *>(a.grad_z) + out0 : nullptr;
@@ -569,7 +574,7 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
     // a chunk's inputs are under way while the chunk after it is computed
     E xn[kMine], dtn[kMine], zn[kMine], gn[kMine];
     f32x4 hn;
-    f32x2 rn;
+    float rn[kShare];
     auto fetch = [&](int c) {
 #pragma unroll
         for (int j = 0; j < kMine; ++j) {
@@ -580,7 +585,8 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
             zn[j] = (zp + tt * z_time)[lo];
             gn[j] = (gp + tt * a.grad_y_time)[lo];
         }
-        rn = rows[(size_t)c * (kChunk * N)];  // (two values per thread are a chunk's rows)
+#pragma unroll
+        for (int j = 0; j < kShare; ++j) rn[j] = rows[(size_t)c * (kChunk * 2 * N) + j * W * kWave];
         hn = reinterpret_cast<const f32x4 *>(a.chunk_states + ((size_t)b * chunks + c) * N * a.dim + (size_t)wave * a.dim * 4)[lo];
     };
     const int c0 = t0 / kChunk;
@@ -605,7 +611,8 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
             s_x[i][lane] = in ? x : 0.f;
             s_gy[i][lane] = in ? gy : 0.f;
         }
-        reinterpret_cast<f32x2 *>(s_rows)[threadIdx.x] = rn;
+#pragma unroll
+        for (int j = 0; j < kShare; ++j) reinterpret_cast<float *>(s_rows)[threadIdx.x + j * W * kWave] = rn[j];
         float h[S] = {hn.x, hn.y, hn.z, hn.w};
         if (c > c0) fetch(c - 1);
         __syncthreads();
@@ -682,11 +689,11 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
                 dbias += ddt;
             }
         }
-        {  // two values per thread are the chunk's shares of dB and dC
-            const int i = threadIdx.x / N, k = threadIdx.x % N;
+#pragma unroll
+        for (int j = 0; j < kShare; ++j) {
+            const int k = threadIdx.x + j * W * kWave, i = k / (2 * N);
             if (tc + i < te)
-                *reinterpret_cast<f32x2 *>(out.BC + (((size_t)b * a.length + tc + i) * g.groups + group) * 2 * N + 2 * k) =
-                    *reinterpret_cast<const f32x2 *>(&s_bc[i][2 * k]);
+                out.BC[(((size_t)b * a.length + tc + i) * g.groups + group) * 2 * N + k % (2 * N)] = s_bc[i][k % (2 * N)];
         }
         __syncthreads();
     }
@@ -1069,9 +1076,9 @@ inline ScanGeom scan_geometry(int batch, int length, int dim) {
     const long long waves = (long long)batch * g.groups;
     const long long want = waves >= 2048 || length <= 64 ? 1 : (10240 + waves - 1) / waves;
     int len = (int)((length + want - 1) / want);
-    const int least = waves * ((length + kChunk - 1) / kChunk) <= 2048 ? kChunk : 2 * kChunk;
+    const int least = waves * ((length + 15) / 16) <= 2048 ? 16 : 32;
     if (len < least) len = least;
-    g.seg_len = (len + kChunk - 1) / kChunk * kChunk;
+    g.seg_len = (len + 15) / 16 * 16;
     g.segments = (length + g.seg_len - 1) / g.seg_len;
     const long long wgs = waves * g.segments;
     g.joined = (int)(wgs > 4096 ? (wgs + 4095) / 4096 : 1);

@@ -142,7 +142,7 @@ Tensor token_embedding_op(const Tensor &tokens_in, const Tensor &weight_in, doub
     TORCH_CHECK_VALUE(weight_in.dim() == 2 && weight_in.size(0) >= 1 && weight_in.size(1) >= 1, "weight must be a non-empty [vocab, dim] tensor");
     TORCH_CHECK_VALUE(tokens_in.numel() >= 1, "tokens must not be empty");
     TORCH_CHECK_VALUE(padding >= -1 && padding < weight_in.size(0), "padding_idx must be None or a row of weight");
-    TORCH_CHECK_VALUE(std::isfinite(scale), "scale must be finite");
+    TORCH_CHECK_VALUE(std::isfinite((float)scale), "scale must be finite in fp32");
     as_int(weight_in.size(0), "vocab");
     as_int(tokens_in.numel() + (1 << 16), "the number of tokens");
     check_on_device(weight_in, "token_embedding");

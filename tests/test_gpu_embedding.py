@@ -157,3 +157,18 @@ def test_tensors_elsewhere_are_refused():
 
     with pytest.raises(RuntimeError, match="tokens must be on"):
         rnnt_amd.token_embedding(torch.zeros(2, dtype=torch.int64), torch.zeros(3, 4, device=DEV))
+
+
+def test_offsets_past_32_bits():
+    """Weight rows, and rows of the gradient, 4 GiB apart."""
+    import rnnt_amd
+
+    tokens, weight, grad = make(300, 2, 64, torch.bfloat16, seed=3)
+    far = 1 << 31
+    pool = torch.empty(far + 4096, dtype=torch.bfloat16, device=DEV)
+    w = pool.as_strided((2, 64), (far, 1), 0)
+    w.copy_(weight)
+    check(tokens, weight, grad, 2.0, None, weight_dev=w)
+    two = pool.as_strided((2, 64), (far, 1), 1024)
+    two.copy_(grad[:2])
+    check(tokens[:2], weight, grad[:2], 2.0, None, grad_dev=two)

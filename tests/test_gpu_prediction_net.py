@@ -65,6 +65,26 @@ def test_forward_and_gradients_against_64_bits(state, width, layers):
         assert err < 2e-5, (k, err)
 
 
+@pytest.mark.parametrize("amp", [torch.bfloat16, torch.float16])
+def test_under_autocast(amp):
+    """fp32 parameters, 16-bit sequences: gradients in fp32, near the fp32 step's."""
+    net = make_net().to(DEV)
+    tokens = torch.randint(0, 29, (3, 9), generator=torch.Generator().manual_seed(1)).to(DEV)
+    go = torch.randn(3, 9, 16, generator=torch.Generator().manual_seed(2)).to(DEV)
+    grads = []
+    for on in (False, True):
+        net.zero_grad()
+        with torch.autocast("cuda", dtype=amp, enabled=on):
+            out, _ = net(tokens)
+        assert out.dtype is (amp if on else torch.float32)
+        out.float().backward(go)
+        grads.append([p.grad.clone() for p in net.parameters()])
+    for (name, _), a, b in zip(net.named_parameters(), *grads):
+        assert b.dtype is torch.float32
+        # a dozen tensors on the way are rounded by half a step of the type each
+        assert float((a - b).norm()) <= 16 * torch.finfo(amp).eps * float(a.norm()) + 1e-6, name
+
+
 def test_hidden_carries_a_sequence_on():
     net = make_net().to(DEV).eval()
     tokens = torch.randint(0, 29, (2, 9), device=DEV)

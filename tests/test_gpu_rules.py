@@ -140,6 +140,23 @@ def test_layouts():
     assert torch.equal(rnnt_amd.process_logits(x.to(DEV), rules).cpu(), plain.rules32(x, 96, **r).to(torch.bfloat16))
 
 
+def test_more_than_32_bits_of_logits():
+    """33 000 rows of 70 001 bf16 logits (4.6 GB): the last rows are what the same rows alone give."""
+    import rnnt_amd
+
+    V, rows = 70001, 33000
+    x = torch.zeros(rows, V, dtype=torch.bfloat16, device=DEV)
+    x[-3:] = torch.randn(3, V, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV).bfloat16()
+    rules = rnnt_amd.LogitRules(bias=torch.linspace(-1, 1, V, device=DEV), history=torch.full((1, 1), 5, dtype=torch.int32, device=DEV),
+                                presence_penalty=3.0)
+    token, logp = rnnt_amd.row_max_logp(x, rules)
+    last = x[-3:].clone()
+    token3, logp3 = rnnt_amd.row_max_logp(last, rules)
+    assert torch.equal(token[-3:], token3) and torch.equal(logp[-3:], logp3) and int(token[0]) == V - 1
+    assert rnnt_amd.process_logits(x, rules, out=x).data_ptr() == x.data_ptr()
+    assert torch.equal(x[-3:], rnnt_amd.process_logits(last, rules))
+
+
 def test_refusals_on_the_device():
     import rnnt_amd
 

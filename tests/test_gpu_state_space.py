@@ -299,6 +299,40 @@ def test_conv_step(dtype, B, D, W):
     assert same.data_ptr() == dev["init"].data_ptr() and torch.equal(dev["init"], state) and torch.equal(y, y2)
 
 
+def test_offsets_past_32_bits():
+    """Two sequences whose rows lie more than 2^32 bytes apart, and steps that far apart: the results of the packed ones."""
+    import rnnt_amd
+
+    far = 1 << 31                                           # elements of bf16: 4 GiB
+    pool = torch.empty(far + (1 << 20), dtype=torch.bfloat16, device=DEV)
+    a, grads = scan_inputs(2, 20, 64, 16, torch.bfloat16, seed=6)
+    dev = {k: v.to(DEV) for k, v in a.items()}
+    gy = grads["gy"].to(DEV)
+    w = torch.randn(64, 4, device=DEV)
+
+    def results(x, B, gy):
+        leaves = [t.detach().requires_grad_(True) for t in (x, B)]
+        y, state = call_scan({**dev, "x": leaves[0], "B": leaves[1]}, None)
+        out = (y, state, *torch.autograd.grad(y, leaves, gy))
+        y, state = rnnt_amd.causal_conv(leaves[0], w)
+        return out + (y, state, torch.autograd.grad(y, leaves[0], gy)[0])
+
+    want = results(dev["x"], dev["B"], gy)
+    views = []
+    for k, (t, at) in enumerate(((dev["x"], 0), (dev["B"], 4096), (gy, 8192))):
+        v = pool.as_strided(t.shape, (far, t.shape[2], 1), at)
+        v.copy_(t)
+        views.append(v)
+    for p, q in zip(want, results(*views)):
+        assert torch.equal(p, q)
+    one = {k: (v[:1, :2] if v.dim() == 3 and k != "init" else v) for k, v in dev.items()}
+    one["init"] = dev["init"][:1]
+    x_far = pool.as_strided((1, 2, 64), (64, far, 1), 0)     # two steps of one sequence
+    x_far.copy_(one["x"])
+    assert all(torch.equal(p, q) for p, q in zip(call_scan(one, None), call_scan({**one, "x": x_far}, None)))
+    assert torch.equal(rnnt_amd.causal_conv(one["x"], w)[0], rnnt_amd.causal_conv(x_far, w)[0])
+
+
 # ---- how they are called -----------------------------------------------------------------------------------------------------
 def test_same_bits_every_time_and_on_another_stream():
     a, grads = scan_inputs(3, 300, 96, 16, torch.bfloat16, seed=7)

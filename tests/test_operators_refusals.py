@@ -52,8 +52,9 @@ def test_embedding_refusals():
     for padding in (5, -1):
         with pytest.raises(ValueError, match="padding_idx"):
             f(t, w, padding_idx=padding)
-    with pytest.raises(ValueError, match="scale"):
-        f(t, w, scale=float("inf"))
+    for scale in (float("inf"), float("nan"), 1e300):
+        with pytest.raises(ValueError, match="scale"):
+            f(t, w, scale=scale)
 
 
 def test_conv_refusals():
