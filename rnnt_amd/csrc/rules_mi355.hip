@@ -210,12 +210,16 @@ __device__ __forceinline__ void store_answer(const RowPart &p, int *out, float *
     logp[r] = nan ? __builtin_nanf("") : (p.m - p.m) - kLn2 * __builtin_amdgcn_logf(p.s);
 }
 
+// Bound by latency: one load of a thread's two pieces behind the counting, then the reduction.  512 rows of 4232 fp32 logits
+// (16 contexts with history, bias and mask) 8 us, one row of 5455 fp16 logits 6 us (10 us by elements, with the whole
+// row off 16 bytes).
 template <typename DT, bool SPLIT>
 __global__ __launch_bounds__(1024) void row_rules_kernel(const typename DT::elem *__restrict__ x, int V, const rnntRules rules,
                                                          int rows_per_context, int *__restrict__ out, float *__restrict__ logp,
                                                          int splits, RowPart *__restrict__ parts) {
     constexpr int E = DT::EPC, kTile = SPLIT ? kTileSplit : kTilePick;
-    __shared__ u32x4 s_words[kTile / 8];
+    extern __shared__ u32x4 s_words[];  // the counts of the row's (the part's) columns: no more than it has, so that short
+                                        // rows share a CU with many others
     __shared__ unsigned long long s_rank[16];
     __shared__ float s_max[16], s_sum[16];
     unsigned *s_count = reinterpret_cast<unsigned *>(s_words);
@@ -297,6 +301,8 @@ __global__ __launch_bounds__(kWave) void row_rules_join_kernel(const RowPart *__
     if (threadIdx.x == 0) store_answer(RowPart{rank, m, s}, out, logp, blockIdx.x);
 }
 
+// Bound by memory once there are rows enough: 64 rows of 70 001 bf16 logits 11 us (37 MB with bias, mask and histories:
+// 3.4 TB/s); a workgroup per row, by elements, took 38.
 template <typename DT>
 __global__ __launch_bounds__(256) void process_logits_kernel(const typename DT::elem *x, int V, const rnntRules rules,
                                                              int rows_per_context, typename DT::elem *processed, int tiles) {
@@ -340,13 +346,9 @@ bool rules_ok(const rnntRules *r, int rows, int V) {
            r->frequency_penalty == r->frequency_penalty;
 }
 
-// Threads of a row's workgroup: about two pieces each; more than 256 leave too few workgroups per CU to hide the
-// counting of one row behind another's reading once there are many rows.
-inline int pick_threads(int rows, int pieces) {
-    int threads = 256;
-    while (threads < 1024 && pieces > 2 * threads && (long long)rows * threads < 512 * 1024) threads *= 2;
-    return threads;
-}
+// Threads of a row's workgroup: one to three pieces each.  1058 pieces (4232 fp32 logits), 512 rows: 8.9, 8.0 and 8.8 us with
+// 256, 512 and 1024 threads; 682 pieces, one row: 7.3, 6.0 and 5.8; 2000 pieces, 16 rows: 12.8, 8.9 and 8.1.
+inline int pick_threads(int rows, int pieces) { return pieces <= 512 ? 256 : (pieces <= 1536 || rows > 256 ? 512 : 1024); }
 
 // 0: a workgroup per row; otherwise workgroups per row.  One workgroup reads a row of 70 001 logits in 24 us whether there
 // is one row or 64; shared out among 18 and joined by a second launch one fp32 row takes 11 us, 64 bf16 rows 15 us.
@@ -360,12 +362,13 @@ rnntStatus_t launch_pick(const void *x, int rows, int V, const rnntRules &r, int
     typedef typename DT::elem E;
     const int splits = pick_splits(V, DT::EPC);
     if (splits == 0) {
-        hipLaunchKernelGGL((row_rules_kernel<DT, false>), dim3(rows), dim3(pick_threads(rows, V / DT::EPC + 1)), 0, st,
+        const size_t counts = r.history ? (((size_t)V + 2 * DT::EPC + 7) & ~(size_t)7) * 2 : 0;  // (whole pieces at both ends)
+        hipLaunchKernelGGL((row_rules_kernel<DT, false>), dim3(rows), dim3(pick_threads(rows, V / DT::EPC + 1)), counts, st,
                            static_cast<const E *>(x), V, r, rows / r.contexts, out, logp, 1, static_cast<RowPart *>(nullptr));
     } else {
         if (workspace == nullptr || !aligned16(workspace) || (long long)rows * splits > 0x7fffffffll) return RNNT_STATUS_INVALID_VALUE;
         RowPart *parts = static_cast<RowPart *>(workspace);
-        hipLaunchKernelGGL((row_rules_kernel<DT, true>), dim3((unsigned)(rows * (long long)splits)), dim3(512), 0, st,
+        hipLaunchKernelGGL((row_rules_kernel<DT, true>), dim3((unsigned)(rows * (long long)splits)), dim3(512), kTileSplit * 2, st,
                            static_cast<const E *>(x), V, r, rows / r.contexts, out, logp, splits, parts);
         hipLaunchKernelGGL(row_rules_join_kernel, dim3(rows), dim3(kWave), 0, st, static_cast<const RowPart *>(parts), splits, out, logp);
     }
