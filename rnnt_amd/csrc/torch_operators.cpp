@@ -9,8 +9,10 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
 #include <cmath>
@@ -73,6 +75,20 @@ bool wants_grad(std::initializer_list<const Tensor *> inputs) {
     for (const Tensor *t : inputs)
         if (t->defined() && t->requires_grad()) return true;
     return false;
+}
+
+// A call that a graph captures, on a leaf that an eager graph made on the default stream still holds: the backward pass would
+// wait for the default stream inside the capture, which ends the process rather than raising.
+void check_capture(std::initializer_list<const Tensor *> inputs, const char *op) {
+    for (const Tensor *t : inputs) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+        if (!accumulator) continue;
+        const auto stream = accumulator->stream();
+        TORCH_CHECK(!stream || stream->id() != 0 || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
+                    "rnnt_amd.", op, " cannot be captured while a graph of an eager call on the default stream holds the same leaf: "
+                    "drop that call's results, or make it on another stream");
+    }
 }
 
 // The gradients as they leave a backward node: differentiating them again raises (there is no second derivative here).
@@ -143,8 +159,11 @@ Tensor token_embedding_op(const Tensor &tokens_in, const Tensor &weight_in, doub
     TORCH_CHECK_VALUE(tokens_in.numel() >= 1, "tokens must not be empty");
     TORCH_CHECK_VALUE(padding >= -1 && padding < weight_in.size(0), "padding_idx must be None or a row of weight");
     TORCH_CHECK_VALUE(std::isfinite((float)scale), "scale must be finite in fp32");
-    as_int(weight_in.size(0), "vocab");
-    as_int(tokens_in.numel() + (1 << 16), "the number of tokens");
+    size_t need = 0;
+    TORCH_CHECK_VALUE(weight_in.size(0) < (1ll << 31) && weight_in.size(1) < (1ll << 31) &&
+                          rnnt_token_embedding_workspace_size(tokens_in.numel(), (int)weight_in.size(0), (int)weight_in.size(1), &need) ==
+                              RNNT_STATUS_SUCCESS,
+                      "too many tokens (at most 2^30), or too large a weight (2^26 rows, 2^21 columns) for one call");
     check_on_device(weight_in, "token_embedding");
     check_same_device(tokens_in, weight_in, "tokens");
     const Tensor tokens = tokens_in.contiguous();
@@ -152,6 +171,7 @@ Tensor token_embedding_op(const Tensor &tokens_in, const Tensor &weight_in, doub
     const bool ordered = weight.size(0) == 1 || weight.stride(0) >= weight.size(1);  // (an expanded weight is laid out first)
     const Tensor w = ordered ? weight : weight.contiguous();
     if (!wants_grad({&w})) return embed_forward(tokens, w, scale);
+    check_capture({&weight_in}, "token_embedding");
     return EmbedFunction::apply(tokens, w, scale, padding);
 }
 
@@ -260,13 +280,32 @@ std::tuple<Tensor, Tensor> causal_conv_op(const Tensor &x_in, const Tensor &weig
     if (bias.defined()) bias = bias.contiguous();
     if (initial.defined()) initial = initial.contiguous();
     if (!wants_grad({&x, &weight, &bias, &initial})) return conv_forward(x, weight, bias, initial, lengths, silu);
+    check_capture({&x_in, &weight_in, &bias, &initial}, "causal_conv");
     const auto out = ConvFunction::apply(x, weight, bias.defined() ? MaybeTensor(bias) : MaybeTensor(),
                                          initial.defined() ? MaybeTensor(initial) : MaybeTensor(), lengths_in, silu);
     return {out[0], out[1]};
 }
 
+// A buffer that the caller gives for a result: nothing that the call reads may lie in it (another thread may read it after it
+// is written), and autograd learns that it changes.
+bool overlap(const Tensor &a, const Tensor &b) {
+    auto end = [](const Tensor &t) {
+        int64_t last = 0;
+        for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+        return static_cast<const char *>(t.data_ptr()) + (last + 1) * t.element_size();
+    };
+    return a.data_ptr() < end(b) && b.data_ptr() < end(a);
+}
+void check_apart(const Tensor &out, std::initializer_list<const Tensor *> inputs, const char *name) {
+    for (const Tensor *t : inputs)
+        TORCH_CHECK_VALUE(!t->defined() || t->numel() == 0 || !overlap(out, *t), name, " must not overlap another argument of the call");
+}
+void changed(const Tensor &out) {
+    if (!out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
+
 // a new state beside the old one, or the caller's buffer
-Tensor state_buffer(const MaybeTensor &out, const Tensor &state) {
+Tensor state_buffer(const MaybeTensor &out, const Tensor &state, std::initializer_list<const Tensor *> others) {
     if (!out.has_value()) return at::empty(state.sizes(), state.options());
     TORCH_CHECK_TYPE(out->scalar_type() == state.scalar_type(), "state_out must have the state's type");
     TORCH_CHECK_VALUE(out->sizes() == state.sizes() && out->is_contiguous() && state.is_contiguous(),
@@ -275,6 +314,8 @@ Tensor state_buffer(const MaybeTensor &out, const Tensor &state) {
     // the very buffer or another one: a buffer that overlaps the state by a part would be read after it is written
     const char *a = static_cast<const char *>(out->data_ptr()), *b = static_cast<const char *>(state.data_ptr());
     TORCH_CHECK_VALUE(a == b || a + out->nbytes() <= b || b + state.nbytes() <= a, "state_out must not overlap the state in part");
+    check_apart(*out, others, "state_out");
+    changed(*out);
     return *out;
 }
 
@@ -296,7 +337,7 @@ std::tuple<Tensor, Tensor> causal_conv_step_op(const Tensor &x_in, const Tensor 
     check_same_device(bias, x_in, "bias");
     check_no_grad({&x_in, &state_in, &weight_in, &bias}, "causal_conv_step");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x_in.device());
-    Tensor out = state_buffer(state_out, state_in);
+    Tensor out = state_buffer(state_out, state_in, {&x_in, &weight_in, &bias});
     const Tensor x = rows_of(x_in), state = state_in.contiguous(), weight = weight_in.contiguous();
     if (bias.defined()) bias = bias.contiguous();
     Tensor y = at::empty(x.sizes(), x.options());
@@ -466,6 +507,7 @@ std::tuple<Tensor, Tensor> selective_scan_op(const Tensor &x, const Tensor &dt, 
         auto out = scan_forward(in, false);
         return {std::get<0>(out), std::get<1>(out)};
     }
+    check_capture({&in.x, &in.dt, &in.A, &in.B, &in.C, &in.D, &in.z, &in.dt_bias, &in.initial}, "selective_scan");
     auto maybe = [](const Tensor &t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
     const auto out = ScanFunction::apply(in.x, in.dt, in.A, in.B, in.C, maybe(in.D), maybe(in.z), maybe(in.dt_bias), maybe(in.initial),
                                          maybe(in.lengths));
@@ -478,7 +520,7 @@ std::tuple<Tensor, Tensor> selective_scan_step_op(const Tensor &x, const Tensor 
     const ScanIn in = scan_check(x, dt, A, B, C, D, z, dt_bias, state, MaybeTensor(), true);
     check_no_grad({&in.x, &in.dt, &in.A, &in.B, &in.C, &in.D, &in.z, &in.dt_bias, &in.initial}, "selective_scan_step");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
-    Tensor out = state_buffer(state_out, state);
+    Tensor out = state_buffer(state_out, state, {&x, &dt, &A, &B, &C, &in.D, &in.z, &in.dt_bias});
     Tensor y = at::empty(x.sizes(), x.options());
     rnntScan a = scan_args(in);
     a.y = y.data_ptr();
@@ -502,6 +544,9 @@ RulesIn rules_check(const Tensor &x, const MaybeTensor &bias_in, const MaybeTens
     in.rows = as_int(x.size(0), "rows");
     TORCH_CHECK_VALUE(x.size(1) <= (1 << 30), "V is too large");
     in.V = (int)x.size(1);
+    size_t need = 0;
+    TORCH_CHECK_VALUE(rnnt_row_rules_workspace_size(in.rows, in.V, dtype_code(x, "x"), &need) == RNNT_STATUS_SUCCESS,
+                      "x has too many rows for one call");
     int64_t contexts = 1;
     const char *by = nullptr;
     auto agree = [&](const Tensor &t, const char *name) {
@@ -592,6 +637,8 @@ Tensor process_logits_op(const Tensor &x, const MaybeTensor &bias, const MaybeTe
         check_same_device(out, x, "out");
         const char *a = static_cast<const char *>(out.data_ptr()), *b = static_cast<const char *>(in.x.data_ptr());
         TORCH_CHECK_VALUE(a == b || a + out.nbytes() <= b || b + in.x.nbytes() <= a, "out must not overlap x in part");
+        check_apart(out, {&in.bias, &in.allowed, &in.history, &in.history_lens}, "out");
+        changed(out);
     } else {
         out = at::empty(in.x.sizes(), in.x.options());
     }

@@ -231,3 +231,49 @@ def test_a_given_history_counts_and_a_callable_mask_is_for_searches():
         rnnt_amd.greedy_search_batch(enc, net, joint, rules=rnnt_amd.LogitRules(bias=torch.zeros(3, device=DEV)))
     with pytest.raises(ValueError, match="rules.history"):
         rnnt_amd.greedy_search_batch(enc, net, joint, rules=rnnt_amd.LogitRules(history=history[:1]))
+
+
+def test_capture_is_refused_while_an_eager_graph_holds_the_parameters():
+    """Refused before anything is launched; once the eager results are gone the same pass is captured and replayed."""
+    import rnnt_amd
+
+    tokens = torch.randint(0, 12, (3, 5), device=DEV)
+    weight = torch.randn(12, 64, device=DEV, requires_grad=True)
+    taps = torch.randn(64, 4, device=DEV, requires_grad=True)
+    dt, A, B = torch.randn(3, 5, 64, device=DEV), -torch.rand(64, 8, device=DEV), torch.randn(3, 5, 8, device=DEV)
+    A.requires_grad_(True)
+
+    def run():
+        x = rnnt_amd.token_embedding(tokens, weight)
+        y, _ = rnnt_amd.causal_conv(x, taps)
+        z, _ = rnnt_amd.selective_scan(y, dt, A, B, B)
+        return (z, *torch.autograd.grad(z, (weight, taps, A), torch.ones_like(z)))
+
+    fixed = torch.randn(3, 5, 64, device=DEV)
+    calls = (lambda: rnnt_amd.token_embedding(tokens, weight), lambda: rnnt_amd.causal_conv(fixed, taps)[0],
+             lambda: rnnt_amd.selective_scan(fixed, dt, A, B, B)[0])
+    for call in calls:
+        held = call()
+        graph, scratch = torch.cuda.CUDAGraph(), torch.zeros(1, device=DEV)
+        with torch.cuda.graph(graph):
+            scratch.add_(1)
+            with pytest.raises(RuntimeError, match="cannot be captured while"):
+                call()
+        del held
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for seed in range(3):
+        tokens.copy_(torch.randint(0, 12, (3, 5), generator=torch.Generator().manual_seed(seed)))
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.default_stream())
+            eager = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, eager))

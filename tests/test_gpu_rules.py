@@ -193,3 +193,34 @@ def test_captured_and_replayed():
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, call()))
+
+
+def test_results_in_the_callers_buffer():
+    """Nothing that the call reads may lie in it, and autograd learns that it changed."""
+    import rnnt_amd
+
+    pool = torch.zeros(4 * 64, device=DEV)
+    x, out = torch.zeros(4, 64, device=DEV), pool.view(4, 64)
+    words = pool.view(torch.int32)
+    for rules in (rnnt_amd.LogitRules(bias=out), rnnt_amd.LogitRules(allowed=words[:2]),
+                  rnnt_amd.LogitRules(history=words[-8:].view(4, 2)),
+                  rnnt_amd.LogitRules(history=torch.zeros(4, 2, dtype=torch.int32, device=DEV), history_lens=words[60:64])):
+        with pytest.raises(ValueError, match="must not overlap another argument"):
+            rnnt_amd.process_logits(x, rules, out=out)
+    leaf = torch.randn(4, 64, device=DEV, requires_grad=True)
+    y = leaf * 2
+    z = y.square().sum()
+    with torch.no_grad():
+        rnnt_amd.process_logits(y, rnnt_amd.LogitRules(presence_penalty=1.0), out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        z.backward()
+    with torch.inference_mode():
+        y = torch.randn(4, 64, device=DEV)
+        assert rnnt_amd.process_logits(y, rnnt_amd.LogitRules(), out=y) is not None
+
+
+def test_history_far_outside_the_vocabulary():
+    x, r = make(2, 1, 37, 12, torch.bfloat16, seed=9)
+    r["history"][:, :4] = torch.tensor([2 ** 31 - 1, -2 ** 31, 2 ** 31 - 8, 37], dtype=torch.int32)
+    r["history_lens"][:] = 12
+    check(x, r)
