@@ -301,7 +301,14 @@ __global__ __launch_bounds__(64) void scan_forward_kernel(const rnntScan a, cons
 // 32 segments of 16 x 1024 x 16 states: 18 us (two reads and a write of 34 MB: 5.6 TB/s); 128 segments of 1536 x 16: 14 us
 // (64 of them, a thread per 4 states and no loads ahead: 24).
 // Up to kJoinAhead segments one wave does it alone, once.
+// A segment's factor exp(A sum_delta) is applied in two halves, each of them at most 2^127: a state may grow (A > 0) from 1e-30
+// by more than fp32 holds, and 0 stays 0 where the factor alone would be infinite.
 constexpr int kJoinWaves = 8, kJoinAhead = 8;
+
+__device__ __forceinline__ float carried(float delta, float half_A2, float h) {
+    const float e = exp2_(fminf(delta * half_A2, 127.f));
+    return e * (e * h);
+}
 
 template <int N, bool BACKWARD, int WAVES>
 __global__ __launch_bounds__(WAVES *kWave) void scan_join_kernel(const rnntScan a, const ScanGeom g) {
@@ -322,7 +329,7 @@ __global__ __launch_bounds__(WAVES *kWave) void scan_join_kernel(const rnntScan 
         if (from) load_row<4>(from + ((size_t)b * a.dim + d) * N + q * 4, start);
     }
 #pragma unroll
-    for (int n = 0; n < 4; ++n) A2[n] *= kLog2e;
+    for (int n = 0; n < 4; ++n) A2[n] *= 0.5f * kLog2e;
     f32x4 *tiles = reinterpret_cast<f32x4 *>(g.seg_state) + ((size_t)b * g.segments * (N / 4) + q) * a.dim + d;
     const float *deltas = g.seg_delta + (size_t)b * g.segments * a.dim + d;
     auto walk = [&](bool write) {
@@ -343,7 +350,7 @@ __global__ __launch_bounds__(WAVES *kWave) void scan_join_kernel(const rnntScan 
                 if (write) tiles[(size_t)s * (N / 4) * a.dim] = f32x4{h[0], h[1], h[2], h[3]};
                 sum += delta[j];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) h[n] = fma_(exp2_(delta[j] * A2[n]), h[n], end[j][n]);
+                for (int n = 0; n < 4; ++n) h[n] = carried(delta[j], A2[n], h[n]) + end[j][n];
             }
         }
         return sum;
@@ -357,7 +364,7 @@ __global__ __launch_bounds__(WAVES *kWave) void scan_join_kernel(const rnntScan 
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
         h[n] = start[n];
-        for (int w = 0; w < wave; ++w) h[n] = fma_(exp2_(s_delta[w][lane] * A2[n]), h[n], s_end[w][n][lane]);
+        for (int w = 0; w < wave; ++w) h[n] = carried(s_delta[w][lane], A2[n], h[n]) + s_end[w][n][lane];
     }
     walk(true);
 }
@@ -502,7 +509,7 @@ struct FoldSteps {
 //   3. each wave adds the waves' shares of its steps and writes dx, ddt, dz.
 // 275 us at the shape above, 28 us for 32 sequences of 41 steps.  Bound by the vector units: some 1600 vector instructions
 // a wave and chunk (17 + 55 a step for 4 states, 18 of them the sums over lanes), issuing 66 % of the time with the two waves
-// per SIMD that 237 registers and 64 KiB of LDS leave.  Chunks of 8 steps leave three (249 us) but keep twice the states for
+// per SIMD that 239 registers and 64 KiB of LDS leave.  Chunks of 8 steps leave three (249 us) but keep twice the states for
 // the backward pass; B and C as scalar operands, each use of which waits for all scalar loads, took 90 us more.
 template <int I>
 struct Index {
@@ -585,7 +592,10 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
             if (dzp) (dzp + (size_t)t * a.dim)[lo] = DT::from_float(0.f);
         }
     }
-    // a chunk's inputs are under way while the chunk after it is computed
+    // A chunk's inputs are under way while the chunk after it is computed.  With 8 states a wave has 8 of its steps, whose inputs
+    // beside a whole chunk of h and decay spill 12 registers; half the walk back there is more room (5; 16 x 1500 x 1024 x 8 bf16, a
+    // training pass: 412 and 385 us; with 16 and 32 states, which do not spill, late loads cost 0.5 %).
+    constexpr bool kLate = N == 8;
     E xn[kMine], dtn[kMine], zn[kMine], gn[kMine];
     f32x4 hn;
     float rn[kShare];
@@ -628,7 +638,7 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
 #pragma unroll
         for (int j = 0; j < kShare; ++j) reinterpret_cast<float *>(s_rows)[threadIdx.x + j * W * kWave] = rn[j];
         float h[S] = {hn.x, hn.y, hn.z, hn.w};
-        if (c > c0) fetch(c - 1);
+        if (!kLate && c > c0) fetch(c - 1);
         __syncthreads();
 
         float before[kChunk][S], decay[kChunk][S];
@@ -650,6 +660,9 @@ __global__ __launch_bounds__(N * 16, 2) void scan_backward_kernel(const rnntScan
         float sums_of[kChunk / 8];
         auto reverse = [&](auto index) {
             constexpr int i = decltype(index)::value;
+            if constexpr (kLate && i == kChunk / 2) {
+                if (c > c0) fetch(c - 1);
+            }
             const f32x4 B = s_rows[i][2 * wave], C = s_rows[i][2 * wave + 1];
             const float delta = s_delta[i][lane], dx = delta * s_x[i][lane], gy = s_gy[i][lane];
             float inner = 0.f, rate = 0.f, sums[2 * S];
@@ -1081,10 +1094,14 @@ inline size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 inline int groups_of(int dim) { return (dim + kWave - 1) / kWave; }
 
+// (A launch has less than 2^32 threads: 16 a state and group of channels in the backward proper, one a value of B and C, and 16 a
+// value of the parameters beside those in the sums.)
 inline bool scan_shape_ok(int batch, int length, int dim, int state) {
-    return batch >= 1 && length >= 1 && dim >= 1 && (state == 8 || state == 16 || state == 32) && length <= (1 << 30) &&
-           (long long)batch * length < (1ll << 31) && (long long)batch * dim * state < (1ll << 31) &&
-           (long long)batch * groups_of(dim) * ((length + kChunk - 1) / kChunk) < (1ll << 31);
+    if (batch < 1 || length < 1 || dim < 1 || (state != 8 && state != 16 && state != 32) || length > (1 << 30)) return false;
+    const long long chunks = (length + kChunk - 1) / kChunk, waves = (long long)batch * groups_of(dim);
+    return (long long)batch * chunks < (1ll << 27) && (long long)batch * dim * state < (1ll << 31) && waves * state < (1ll << 28) &&
+           waves * chunks < (1ll << 31) &&
+           (batch * chunks * kChunk + 1) * 2 * state + ((long long)dim * (state + 2) + 4 * kWave) * 16 < (1ll << 32);
 }
 
 // Segments: none while the (sequence, 64 channels) pairs alone fill the chip.
@@ -1229,7 +1246,7 @@ inline long long conv_items(int batch, int length, int run) {  // workgroups per
 inline bool conv_shape_ok(int batch, int length, int dim, int width) {
     return batch >= 1 && length >= 1 && dim >= 1 && width >= 2 && width <= 4 && length <= (1 << 30) &&
            (long long)batch * length < (1ll << 31) && (long long)batch * dim < (1ll << 31) &&
-           (long long)dim * 8 < (1ll << 31) && conv_items(batch, length, kRunForward) * groups_of(dim) < (1ll << 31);
+           dim < (1 << 25) && conv_items(batch, length, kRunForward) * groups_of(dim) < (1ll << 24);  // (less than 2^32 threads)
 }
 
 template <typename DT, int W>

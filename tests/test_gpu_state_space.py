@@ -421,3 +421,68 @@ def test_refusals_on_the_device():
             rnnt_amd.selective_scan_step(*row, state.cpu())
         with pytest.raises(RuntimeError, match="lengths must be on"):
             rnnt_amd.selective_scan(a["x"], a["dt"], a["A"], a["B"], a["C"], lengths=torch.zeros(2, dtype=torch.int32))
+
+
+def test_scan_of_growing_states_over_segments():
+    """A > 0: over 16 steps the states grow by e^96, more than fp32 holds, from 1e-30; and zeros stay zeros.  The exponent of 96 is off by
+    7 * 96 u from its steps and, where a segment's steps are added up first, by 16 u of it; 96 steps of 3 roundings: 2500 u of a
+    value that is carried once, twice that for products of a state and a gradient."""
+    L, D, N = 96, 4, 8
+    a, grads = scan_inputs(1, L, D, N, torch.float32, seed=21)
+    a["A"].fill_(1.0)
+    a["bias"].zero_()
+    a["dt"].fill_(-200.0)
+    a["dt"][:, 32:48] = 6.0
+    a["x"].zero_()
+    a["init"] *= 1e-30
+    a["init"][:, 1] = 0.0
+    grads = {k: v * 1e-30 for k, v in grads.items()}
+    dev = {k: v.to(DEV).requires_grad_(True) for k, v in a.items()}
+    y, state = call_scan(dev, None)
+    got = torch.autograd.grad([y, state], list(dev.values()), [grads["gy"].to(DEV), grads["gfinal"].to(DEV)])
+    ref, mag = (plain.scan(**{k: v.double() for k, v in a.items()}, lens=None, gy=grads["gy"].double(), gfinal=grads["gfinal"].double(),
+                           magnitude=m) for m in (False, True))
+    assert float(ref["state"].abs().max()) > 1e10 and torch.count_nonzero(state[:, 1]) == 0
+    plain.assert_within(y, ref["y"], 2500 * U * mag["y"] + 1e-37, "y")
+    plain.assert_within(state, ref["state"], 2500 * U * mag["state"] + 1e-37, "state")
+    for k, g in zip(dev, got):
+        plain.assert_within(g, ref["d" + k], 5000 * U * mag["d" + k] + 1e-37, "d" + k)
+
+
+def test_results_in_the_callers_buffer():
+    """Nothing that a step reads may lie in it, and autograd learns that it changed."""
+    import rnnt_amd
+
+    a = {k: v.to(DEV) for k, v in scan_inputs(2, 1, 8, 8, torch.float32)[0].items()}
+    row = [a[k][:, 0] for k in ("x", "dt")] + [a["A"]] + [a[k][:, 0] for k in ("B", "C")]
+    kept = a["init"].clone().requires_grad_(True) * 1
+    z = kept.square().sum()
+    with torch.no_grad():
+        for i in (0, 1, 2, 3, 4):
+            out = torch.zeros(2, 8, 8, device=DEV)
+            args = list(row)
+            args[i] = out.view(-1)[-args[i].numel():].view(args[i].shape)
+            with pytest.raises(ValueError, match="state_out must not overlap another argument"):
+                rnnt_amd.selective_scan_step(*args, a["init"], state_out=out)
+        conv = torch.zeros(2, 3, 8, device=DEV)
+        w = torch.randn(8, 4, device=DEV)
+        with pytest.raises(ValueError, match="state_out must not overlap another argument"):
+            rnnt_amd.causal_conv_step(conv[:, 1], torch.zeros(2, 3, 8, device=DEV), w, state_out=conv)
+        want = rnnt_amd.selective_scan_step(*row, kept.clone())[1]
+        _, state = rnnt_amd.selective_scan_step(*row, kept, state_out=kept)
+        assert state.data_ptr() == kept.data_ptr() and torch.equal(kept, want)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        z.backward()
+
+
+def test_backward_twice_gives_the_same_bits():
+    import rnnt_amd
+
+    a, grads = scan_inputs(2, 150, 64, 16, torch.bfloat16, seed=8)
+    dev = {k: v.to(DEV).requires_grad_(True) for k, v in a.items()}
+    w = torch.randn(64, 4, device=DEV, requires_grad=True)
+    x, _ = rnnt_amd.causal_conv(dev["x"], w)
+    y, _ = call_scan({**dev, "x": x}, None)
+    leaves = [*dev.values(), w]
+    first, again = (torch.autograd.grad(y, leaves, grads["gy"].to(DEV), retain_graph=True) for _ in range(2))
+    assert all(torch.equal(p, q) for p, q in zip(first, again))
