@@ -397,7 +397,7 @@ rnntStatus_t rnnt_row_max_logp(const void *x, int rows, int V, rnntDtype_t dtype
  * token 0 and a NaN score, as a row of -inf there.  rnnt_process_logits writes x' itself, rounded to the logits' type
  * once; processed may be x (in place).
  * history_stride <= RNNT_MAX_HISTORY (the counters hold 16 bits).  workspace: rnnt_row_rules_workspace_size bytes (0 for
- * rows of ordinary length: NULL then), 16-byte aligned.  V <= 2^30.
+ * rows of ordinary length: NULL then), 16-byte aligned.  V <= 2^30, rows * (V / 4096 + 2) < 2^23.
  */
 #define RNNT_MAX_HISTORY 65535
 typedef struct {
@@ -427,7 +427,7 @@ rnntStatus_t rnnt_process_logits(const void *x, int rows, int V, rnntDtype_t dty
  * position order, fp32), rounded once, for EVERY v in [0, vocab): zeros where no position holds v, and for
  * v = padding_idx (-1: none); tokens outside [0, vocab) add nothing.  grad_out rows are grad_stride elements apart.  No
  * atomics.  workspace: rnnt_token_embedding_workspace_size bytes, 16-byte aligned (0 for short sequences: NULL then).
- * n < 2^31 - 2^16.
+ * n <= 2^30, vocab <= 2^26, dim <= 2^21.
  */
 rnntStatus_t rnnt_token_embedding_forward(const void *tokens, int tokens_64, long long n, const void *weight,
                                           long long weight_stride, int vocab, int dim, float scale, rnntDtype_t dtype,

@@ -25,6 +25,7 @@ constexpr int kListRows = 16, kListWaves = 8, kListAlone = 64;
 constexpr int kRankMax = 4096;    // up to this many positions are sorted by counting smaller ones
 constexpr int kRankRows = 64;     // rows of the gradient that a workgroup of the counting kernel clears
 constexpr int kSortItems = 1024;  // positions per workgroup and pass of the radix sort
+constexpr int kSortMany = 3 << 17;  // from so many positions on the workgroups' counts are summed by a launch of their own
 constexpr int kJoinWaves = 8, kJoinAlone = 64;
 constexpr int kDigits = 256;
 
@@ -152,6 +153,9 @@ __global__ __launch_bounds__(kBlock) void embed_rank_kernel(const void *__restri
 // Many positions: radix sort from the lowest digit, 8 bits per pass, two launches per pass (65 408 positions: 4 + 7 us the
 // first pass, 4 + 8 us the second; bound by the launches' latencies, not by their 0.5 MB).  A workgroup's wave w owns
 // its w-th quarter; lanes with the same digit find each other with 8 ballots, so that ranks follow the position.
+// A workgroup adds up the counts of those before it itself, which is quadratic in their number: from kSortMany positions
+// on a launch between the two forms the sums (MANY).  Whole backward passes of 64 fp32 columns, without and with it: 262 144
+// positions 56 and 64 us, 524 288 82 and 70, 4 194 304 1477 and 458.
 template <bool FIRST>
 __device__ __forceinline__ int sort_key(const void *src, int tokens_64, long long i, int vocab, long long padding) {
     return FIRST ? key_at(src, tokens_64, i, vocab, padding) : static_cast<const int *>(src)[i];
@@ -170,6 +174,33 @@ __global__ __launch_bounds__(kBlock) void embed_digit_kernel(const void *__restr
     counts[(size_t)blockIdx.x * kDigits + threadIdx.x] = s_count[threadIdx.x];
 }
 
+// counts[w][digit] <- the sum over the workgroups before w, counts[parts][digit] <- over all; a workgroup per digit, its
+// threads a range each.
+__global__ __launch_bounds__(kBlock) void embed_prefix_kernel(int *__restrict__ counts, int parts) {
+    __shared__ int s_sum[kBlock];
+    const int per = (parts + kBlock - 1) / kBlock;
+    const int w0 = (int)threadIdx.x * per < parts ? (int)threadIdx.x * per : parts, w1 = w0 + per < parts ? w0 + per : parts;
+    int *column = counts + blockIdx.x;
+    int sum = 0;
+#pragma unroll 8
+    for (int w = w0; w < w1; ++w) sum += column[(size_t)w * kDigits];
+    s_sum[threadIdx.x] = sum;
+    __syncthreads();
+    for (int step = 1; step < kBlock; step <<= 1) {
+        const int v = (int)threadIdx.x >= step ? s_sum[threadIdx.x - step] : 0;
+        __syncthreads();
+        s_sum[threadIdx.x] += v;
+        __syncthreads();
+    }
+    int before = s_sum[threadIdx.x] - sum;
+    for (int w = w0; w < w1; ++w) {
+        const int c = column[(size_t)w * kDigits];
+        column[(size_t)w * kDigits] = before;
+        before += c;
+    }
+    if (threadIdx.x == kBlock - 1) column[(size_t)parts * kDigits] = before;
+}
+
 __device__ __forceinline__ unsigned long long same_digit(int digit, bool live) {
     unsigned long long peers = __ballot(live);
 #pragma unroll
@@ -180,7 +211,7 @@ __device__ __forceinline__ unsigned long long same_digit(int digit, bool live) {
     return peers;
 }
 
-template <bool FIRST>
+template <bool FIRST, bool MANY>
 __global__ __launch_bounds__(kBlock) void embed_place_kernel(const void *__restrict__ src, int tokens_64, int n, int vocab,
                                                              long long padding, int bit, const int *__restrict__ counts,
                                                              const int *__restrict__ order_in, int *__restrict__ sorted,
@@ -191,11 +222,16 @@ __global__ __launch_bounds__(kBlock) void embed_place_kernel(const void *__restr
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     const long long base = (long long)blockIdx.x * kSortItems + wave * (kSortItems / kWaves);
     int before = 0, total = 0;  // of digit threadIdx.x: in the workgroups before this one, in all
+    if constexpr (MANY) {
+        before = counts[(size_t)blockIdx.x * kDigits + threadIdx.x];
+        total = counts[(size_t)gridDim.x * kDigits + threadIdx.x];
+    } else {
 #pragma unroll 16
-    for (int w = 0; w < (int)gridDim.x; ++w) {
-        const int c = counts[(size_t)w * kDigits + threadIdx.x];
-        before += w < (int)blockIdx.x ? c : 0;
-        total += c;
+        for (int w = 0; w < (int)gridDim.x; ++w) {
+            const int c = counts[(size_t)w * kDigits + threadIdx.x];
+            before += w < (int)blockIdx.x ? c : 0;
+            total += c;
+        }
     }
     s_total[threadIdx.x] = total;
 #pragma unroll
@@ -567,14 +603,15 @@ inline EmbedSpace embed_space(long long n, int vocab, int dim) {
         s.sorted[i] = take((size_t)n * 4);
         s.order[i] = take((size_t)n * 4);
     }
-    if (n > kRankMax) s.counts = take((size_t)sort_blocks(n) * kDigits * 4);
+    if (n > kRankMax) s.counts = take((size_t)(sort_blocks(n) + 1) * kDigits * 4);
     s.partial = take((size_t)pieces_of(n) * 2 * dim * 4);
     s.total = at;
     return s;
 }
 
+// (positions are added in 32 bits, and a launch has less than 2^32 threads: 32 to a row of the vocabulary at most)
 inline bool embed_shape_ok(long long n, int vocab, int dim) {
-    return n >= 1 && n < (1ll << 31) - (1 << 16) && vocab >= 1 && vocab < 0x7fffffff && dim >= 1 && dim <= (1 << 21);
+    return n >= 1 && n <= (1ll << 30) && vocab >= 1 && vocab <= (1 << 26) && dim >= 1 && dim <= (1 << 21);
 }
 
 // lanes that share a row: a power of two that covers the row's pieces, at most a wave
@@ -588,17 +625,42 @@ template <typename DT>
 rnntStatus_t embed_forward(const void *tokens, int tokens_64, long long n, const void *weight, long long weight_stride, int vocab,
                            int dim, float scale, void *out, hipStream_t st) {
     typedef typename DT::elem E;
+    constexpr long long kForwardRows = 1ll << 25;  // rows of one launch, of at most 64 threads each
     const bool vec = dim % DT::EPC == 0 && weight_stride % DT::EPC == 0 && aligned16(weight) && aligned16(out);
     const int shift = row_shift(dim, vec ? DT::EPC : 1);
-    const long long blocks = ((n << shift) + kBlock - 1) / kBlock;
-    if (blocks > 0x7fffffffll) return RNNT_STATUS_INVALID_VALUE;
-    if (vec)
-        hipLaunchKernelGGL((embed_forward_kernel<DT, DT::EPC>), dim3((unsigned)blocks), dim3(kBlock), 0, st, tokens, tokens_64, n,
-                           static_cast<const E *>(weight), weight_stride, vocab, dim, scale, static_cast<E *>(out), shift);
-    else
-        hipLaunchKernelGGL((embed_forward_kernel<DT, 1>), dim3((unsigned)blocks), dim3(kBlock), 0, st, tokens, tokens_64, n,
-                           static_cast<const E *>(weight), weight_stride, vocab, dim, scale, static_cast<E *>(out), shift);
+    for (long long at = 0; at < n; at += kForwardRows) {
+        const long long rows = n - at < kForwardRows ? n - at : kForwardRows;
+        const dim3 blocks((unsigned)(((rows << shift) + kBlock - 1) / kBlock));
+        const void *tok = static_cast<const char *>(tokens) + at * (tokens_64 ? 8 : 4);
+        E *o = static_cast<E *>(out) + at * dim;
+        if (vec)
+            hipLaunchKernelGGL((embed_forward_kernel<DT, DT::EPC>), blocks, dim3(kBlock), 0, st, tok, tokens_64, rows,
+                               static_cast<const E *>(weight), weight_stride, vocab, dim, scale, o, shift);
+        else
+            hipLaunchKernelGGL((embed_forward_kernel<DT, 1>), blocks, dim3(kBlock), 0, st, tok, tokens_64, rows,
+                               static_cast<const E *>(weight), weight_stride, vocab, dim, scale, o, shift);
+    }
     return hipGetLastError() == hipSuccess ? RNNT_STATUS_SUCCESS : RNNT_STATUS_EXECUTION_FAILED;
+}
+
+// gives which of the two buffers holds the result
+template <bool MANY>
+int radix_sort(const void *tokens, int tokens_64, int n, int vocab, long long padding, int *counts, int *const *sorted, int *const *order,
+               hipStream_t st) {
+    const int parts = sort_blocks(n);
+    int at = 0;
+    for (int bit = 0; bit == 0 || (bit < 31 && (vocab >> bit) != 0); bit += 8) {
+        const void *src = bit == 0 ? tokens : sorted[at];
+        const int to = bit == 0 ? 0 : 1 - at;
+        hipLaunchKernelGGL((bit == 0 ? embed_digit_kernel<true> : embed_digit_kernel<false>), dim3(parts), dim3(kBlock), 0, st,
+                           src, tokens_64, n, vocab, padding, bit, counts);
+        if (MANY) hipLaunchKernelGGL(embed_prefix_kernel, dim3(kDigits), dim3(kBlock), 0, st, counts, parts);
+        hipLaunchKernelGGL((bit == 0 ? embed_place_kernel<true, MANY> : embed_place_kernel<false, MANY>), dim3(parts), dim3(kBlock), 0, st,
+                           src, tokens_64, n, vocab, padding, bit, static_cast<const int *>(counts),
+                           static_cast<const int *>(order[at]), sorted[to], order[to]);
+        at = to;
+    }
+    return at;
 }
 
 template <typename DT, int VEC>
@@ -627,24 +689,13 @@ rnntStatus_t embed_backward_with(const void *tokens, int tokens_64, int n, const
                            n, vocab, padding, sorted[0], order[0], grad_weight, dim, blocks);
     } else {
         int *counts = reinterpret_cast<int *>(ws + sp.counts);
-        const dim3 grid((unsigned)sort_blocks(n));
-        hipLaunchKernelGGL((embed_digit_kernel<true>), grid, dim3(kBlock), 0, st, tokens, tokens_64, n, vocab, padding, 0, counts);
-        hipLaunchKernelGGL((embed_place_kernel<true>), grid, dim3(kBlock), 0, st, tokens, tokens_64, n, vocab, padding, 0,
-                           static_cast<const int *>(counts), static_cast<const int *>(nullptr), sorted[0], order[0]);
-        for (int bit = 8; bit < 31 && (vocab >> bit) != 0; bit += 8) {
-            hipLaunchKernelGGL((embed_digit_kernel<false>), grid, dim3(kBlock), 0, st, static_cast<const void *>(sorted[at]), 0, n, vocab,
-                               padding, bit, counts);
-            hipLaunchKernelGGL((embed_place_kernel<false>), grid, dim3(kBlock), 0, st, static_cast<const void *>(sorted[at]), 0, n, vocab,
-                               padding, bit, static_cast<const int *>(counts), static_cast<const int *>(order[at]), sorted[1 - at],
-                               order[1 - at]);
-            at = 1 - at;
-        }
+        at = (n >= kSortMany ? radix_sort<true> : radix_sort<false>)(tokens, tokens_64, n, vocab, padding, counts, sorted, order, st);
     }
     const int shift = row_shift(dim, VEC), piece = piece_of(n), pieces = pieces_of(n);
     const int slices = (dim + (VEC << shift) - 1) / (VEC << shift);
     const long long blocks = ((((long long)pieces * slices) << shift) + kBlock - 1) / kBlock;
     const long long zero_blocks = n <= kRankMax ? 0 : ((vocab - 1) / 16 / (kBlock / kWave)) + 1;
-    if (blocks + zero_blocks > 0x7fffffffll) return RNNT_STATUS_INVALID_VALUE;
+    if ((blocks + zero_blocks) * kBlock >= 1ll << 32) return RNNT_STATUS_INVALID_VALUE;
     hipLaunchKernelGGL((embed_sum_kernel<DT, VEC>), dim3((unsigned)(blocks + zero_blocks)), dim3(kBlock), 0, st,
                        static_cast<const int *>(sorted[at]), static_cast<const int *>(order[at]), n, grad, grad_stride, vocab, dim, scale,
                        grad_weight, partial, piece, pieces, slices, shift, (unsigned)blocks);

@@ -147,8 +147,10 @@ __device__ __forceinline__ void count_history(unsigned *s_count, const int *hist
     for (int i = threadIdx.x; i < slots / 2; i += blockDim.x) s_count[i] = 0u;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        const int v = history[i], k = v + off - first;
-        if (v >= 0 && v < V && k >= 0 && k < slots) atomicAdd(&s_count[k >> 1], 1u << ((k & 1) * 16));
+        const int v = history[i];
+        if (v < 0 || v >= V) continue;
+        const int k = v + off - first;
+        if (k >= 0 && k < slots) atomicAdd(&s_count[k >> 1], 1u << ((k & 1) * 16));
     }
     __syncthreads();
 }
@@ -337,6 +339,11 @@ __global__ __launch_bounds__(256) void process_logits_kernel(const typename DT::
     }
 }
 
+// (a launch has less than 2^32 threads: at most 512 to 4096 columns where there are many rows)
+inline bool rows_ok(int rows, int V) {
+    return rows >= 1 && V >= 1 && V <= 0x40000000 && (long long)rows * (V / kTileSplit + 2) < (1ll << 23);
+}
+
 bool rules_ok(const rnntRules *r, int rows, int V) {
     if (r == nullptr || r->contexts < 1 || rows % r->contexts != 0) return false;
     if (r->history && (r->history_stride < 1 || r->history_stride > RNNT_MAX_HISTORY)) return false;
@@ -366,7 +373,7 @@ rnntStatus_t launch_pick(const void *x, int rows, int V, const rnntRules &r, int
         hipLaunchKernelGGL((row_rules_kernel<DT, false>), dim3(rows), dim3(pick_threads(rows, V / DT::EPC + 1)), counts, st,
                            static_cast<const E *>(x), V, r, rows / r.contexts, out, logp, 1, static_cast<RowPart *>(nullptr));
     } else {
-        if (workspace == nullptr || !aligned16(workspace) || (long long)rows * splits > 0x7fffffffll) return RNNT_STATUS_INVALID_VALUE;
+        if (workspace == nullptr || !aligned16(workspace)) return RNNT_STATUS_INVALID_VALUE;
         RowPart *parts = static_cast<RowPart *>(workspace);
         hipLaunchKernelGGL((row_rules_kernel<DT, true>), dim3((unsigned)(rows * (long long)splits)), dim3(512), kTileSplit * 2, st,
                            static_cast<const E *>(x), V, r, rows / r.contexts, out, logp, splits, parts);
@@ -379,7 +386,6 @@ template <typename DT>
 rnntStatus_t launch_process(const void *x, int rows, int V, const rnntRules &r, void *processed, hipStream_t st) {
     typedef typename DT::elem E;
     const long long tiles = ((long long)V + DT::EPC - 1 + kTileOut - 1) / kTileOut;  // (a row's pieces may begin up to EPC - 1 before it)
-    if (tiles * rows > 0x7fffffffll) return RNNT_STATUS_INVALID_VALUE;
     hipLaunchKernelGGL((process_logits_kernel<DT>), dim3((unsigned)(tiles * rows)), dim3(256), 0, st, static_cast<const E *>(x), V, r,
                        rows / r.contexts, static_cast<E *>(processed), (int)tiles);
     return hipGetLastError() == hipSuccess ? RNNT_STATUS_SUCCESS : RNNT_STATUS_EXECUTION_FAILED;
@@ -390,7 +396,7 @@ rnntStatus_t launch_process(const void *x, int rows, int V, const rnntRules &r, 
 extern "C" {
 
 rnntStatus_t rnnt_row_rules_workspace_size(int rows, int V, rnntDtype_t dtype, size_t *size_bytes) {
-    if (size_bytes == nullptr || rows < 1 || V < 1 || V > 0x40000000 || dtype < RNNT_DTYPE_F32 || dtype > RNNT_DTYPE_F16)
+    if (size_bytes == nullptr || !rows_ok(rows, V) || dtype < RNNT_DTYPE_F32 || dtype > RNNT_DTYPE_F16)
         return RNNT_STATUS_INVALID_VALUE;
     *size_bytes = (size_t)rows * pick_splits(V, dtype == RNNT_DTYPE_F32 ? F32::EPC : F16::EPC) * sizeof(RowPart);
     return RNNT_STATUS_SUCCESS;
@@ -398,7 +404,7 @@ rnntStatus_t rnnt_row_rules_workspace_size(int rows, int V, rnntDtype_t dtype, s
 
 rnntStatus_t rnnt_row_rules(const void *x, int rows, int V, rnntDtype_t dtype, const rnntRules *rules, int *out, float *logp,
                             void *workspace, void *stream) {
-    if (x == nullptr || out == nullptr || rows < 1 || V < 1 || V > 0x40000000 || !rules_ok(rules, rows, V)) return RNNT_STATUS_INVALID_VALUE;
+    if (x == nullptr || out == nullptr || !rows_ok(rows, V) || !rules_ok(rules, rows, V)) return RNNT_STATUS_INVALID_VALUE;
     hipStream_t st = static_cast<hipStream_t>(stream);
     switch (dtype) {
         case RNNT_DTYPE_F32: return launch_pick<F32>(x, rows, V, *rules, out, logp, workspace, st);
@@ -410,7 +416,7 @@ rnntStatus_t rnnt_row_rules(const void *x, int rows, int V, rnntDtype_t dtype, c
 
 rnntStatus_t rnnt_process_logits(const void *x, int rows, int V, rnntDtype_t dtype, const rnntRules *rules, void *processed,
                                  void *stream) {
-    if (x == nullptr || processed == nullptr || rows < 1 || V < 1 || V > 0x40000000 || !rules_ok(rules, rows, V)) return RNNT_STATUS_INVALID_VALUE;
+    if (x == nullptr || processed == nullptr || !rows_ok(rows, V) || !rules_ok(rules, rows, V)) return RNNT_STATUS_INVALID_VALUE;
     hipStream_t st = static_cast<hipStream_t>(stream);
     switch (dtype) {
         case RNNT_DTYPE_F32: return launch_process<F32>(x, rows, V, *rules, processed, st);

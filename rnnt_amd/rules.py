@@ -100,6 +100,11 @@ class HistoryRules:
         before = 0 if rules.history is None else rules.history.shape[-1]
         if rules.history is not None and (rules.history.dim() != 2 or rules.history.shape[0] != batch):
             raise ValueError(f"rules.history must be [{batch}, n]")
+        if rules.history_lens is not None and (rules.history is None or rules.history_lens.shape != (batch,)):
+            raise ValueError(f"rules.history_lens must be [{batch}], beside a history")
+        for name in ("history", "history_lens"):
+            if getattr(rules, name) is not None and getattr(rules, name).dtype is not torch.int32:
+                raise TypeError(f"rules.{name} must be torch.int32")
         if before + most > 65535:
             raise ValueError("the history (with one token per frame) is longer than 65535 tokens")
         self.history = torch.full((batch, before + most), -1, dtype=torch.int32, device=device)   # -1: no token

@@ -172,3 +172,37 @@ def test_offsets_past_32_bits():
     two = pool.as_strided((2, 64), (far, 1), 1024)
     two.copy_(grad[:2])
     check(tokens[:2], weight, grad[:2], 2.0, None, grad_dev=two)
+
+
+@pytest.mark.parametrize("n,V", [((3 << 17) - 1, 300), (3 << 17, 300), (500_001, 70_000), ((1 << 21) + 77, 65_537)])
+def test_many_positions(n, V):
+    """Both ways of the sort: workgroups that add up the counts before them, and counts summed by a launch of their own."""
+    check(*make(n, V, 4, torch.float32, seed=n), scale=1.0, padding=0)
+
+
+def test_more_rows_than_one_launch_takes():
+    """A lane per element and 64 lanes to a row: 2^25 rows a launch."""
+    import rnnt_amd
+
+    n, g = (1 << 25) + 3, torch.Generator(device=DEV).manual_seed(4)
+    weight = torch.randn(11, 33, generator=g, device=DEV).bfloat16()
+    for index in (torch.int32, torch.int64):
+        tokens = torch.randint(0, 11, (n,), generator=g, device=DEV, dtype=index)
+        out = rnnt_amd.token_embedding(tokens, weight, 2.0)
+        for part in (slice(0, 1000), slice(n - 1000, n)):
+            assert torch.equal(out[part], weight[tokens[part].long()] * 2)      # (times 2: exact)
+        assert torch.equal(out.view(torch.int16).sum(1, dtype=torch.int64),
+                           (weight * 2).view(torch.int16).sum(1, dtype=torch.int64)[tokens.long()])
+
+
+def test_backward_twice_and_after_the_tokens_changed():
+    import rnnt_amd
+
+    tokens, weight, grad = (t.to(DEV) for t in make(300, 20, 8, torch.float32))
+    w = weight.requires_grad_(True)
+    out = rnnt_amd.token_embedding(tokens, w)
+    first, again = (torch.autograd.grad(out, w, grad, retain_graph=True)[0] for _ in range(2))
+    assert torch.equal(first, again)
+    tokens.add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(out, w, grad)

@@ -315,3 +315,45 @@ def test_plain_conv_gradient_against_differences():
         live = (torch.arange(6)[None] < torch.tensor(lens)[:, None]).double()[..., None]
         _directional(lambda i: plain.conv(i["x"], i["w"], i["b"], i["init"], lens, silu), a, {k: o["d" + k] for k in a},
                      dict(y=gy * live, state=gf))
+
+
+def test_calls_beyond_a_launch_are_refused():
+    """A launch has less than 2^32 threads, and positions are added in 32 bits."""
+    one = torch.zeros(1, 1)
+    with pytest.raises(ValueError, match="too many tokens"):
+        rnnt_amd.token_embedding(torch.zeros(1, dtype=I32).expand((1 << 30) + 1), one)
+    with pytest.raises(ValueError, match="too large a weight"):
+        rnnt_amd.token_embedding(torch.zeros(1, dtype=I32), one.expand((1 << 26) + 1, 1))
+    with pytest.raises(ValueError, match="too large a weight"):
+        rnnt_amd.token_embedding(torch.zeros(1, dtype=I32), one.expand(1, (1 << 21) + 1))
+    for rows, V in ((1 << 22, 1), (1 << 18, 70001 * 2)):
+        with pytest.raises(ValueError, match="too many rows"):
+            rnnt_amd.row_argmax(one.expand(rows, V), rnnt_amd.LogitRules())
+    for B, L, D in ((1 << 24, 1, 64), (1, 1 << 27, 1), (4, 1, 1 << 25)):
+        x = one.expand(B, L, D)
+        bc = one.expand(B, L, 16)
+        with pytest.raises(ValueError, match="too large for one call"):
+            rnnt_amd.selective_scan(x, x, one.expand(D, 16), bc, bc)
+    for B, L, D in ((1 << 27, 1, 1), (1, 1, 1 << 25)):
+        with pytest.raises(ValueError, match="too large for one call"):
+            rnnt_amd.causal_conv(one.expand(B, L, D), one.expand(D, 4))
+
+
+def test_search_rules_are_checked():
+    from rnnt_amd.rules import HistoryRules
+
+    R = rnnt_amd.LogitRules
+    history, lens = torch.tensor([[3, 4], [5, 6]], dtype=I32), torch.tensor([2, 1], dtype=I32)
+    kept = HistoryRules(R(history=history, history_lens=lens), 2, 9, 4, "cpu")
+    kept.emit([1], [7])
+    assert kept.of([0, 1]).history.tolist() == [[3, 4, -1], [5, -1, 7]]
+    for bad, error in ((R(history=history.long()), TypeError), (R(history=history, history_lens=lens.long()), TypeError),
+                       (R(history=history, history_lens=lens[:1]), ValueError), (R(history_lens=lens), ValueError),
+                       (R(history=history[:1]), ValueError), (R(bias=torch.zeros(8)), ValueError),
+                       (R(allowed=lambda tokens: torch.zeros(2, dtype=I32)), ValueError), (R(history=history), None)):
+        if error is None:
+            with pytest.raises(ValueError, match="longer than 65535"):
+                HistoryRules(bad, 2, 9, 65534, "cpu")
+            continue
+        with pytest.raises(error):
+            HistoryRules(bad, 2, 9, 4, "cpu")
