@@ -138,11 +138,11 @@ _lock = threading.Lock()
 _lib = None
 
 
-def build(verbose: bool = False) -> str:
-    """Compile the HIP library for gfx950 (cross-compiles without a GPU)."""
+def build(verbose: bool = False, force: bool = False) -> str:
+    """Compile the HIP library for gfx950 (cross-compiles without a GPU); ``force``: every source, changed or not."""
     out = None if verbose else subprocess.DEVNULL
     # PYTHON: the compiled binding must be built against the torch of the interpreter that will load it
-    subprocess.check_call(["make", "-C", CSRC_DIR, "PYTHON=" + sys.executable], stdout=out)
+    subprocess.check_call(["make", "-C", CSRC_DIR, "PYTHON=" + sys.executable] + (["-B", "-j4"] if force else []), stdout=out)
     return LIB_PATH
 
 
