@@ -853,8 +853,9 @@ __device__ __forceinline__ float conv_in(const rnntConv &c, int b, long long t, 
     return c.initial_state ? DT::to_float(static_cast<const E *>(c.initial_state)[((size_t)b * (W - 1) + (W - 1 + t)) * c.dim + d]) : 0.f;
 }
 
-// Bound by memory: 16 x 1500 x 1024 fp16 (62 % of the steps live) 20 us, 80 MB at 4 TB/s.
-template <typename DT, int W>
+// Bound by memory: 16 x 1500 x 1024 fp16 (62 % of the steps live) 16.5 us, 80 MB at 4.8 TB/s (20 us with a test per step: whole
+// blocks and the activation as a constant leave none).
+template <typename DT, int W, bool SILU>
 __global__ __launch_bounds__(kConvWaves *kWave) void conv_forward_kernel(const rnntConv c, int runs, int groups) {
     typedef typename DT::elem E;
     const int lane = threadIdx.x & (kWave - 1);
@@ -878,26 +879,32 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_forward_kernel(const r
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) win[k + 1] = conv_in<DT, W>(c, (int)b, (long long)t0 - (W - 1) + k, d);
     }
-    for (int tb = t0; tb < te; tb += kConvAhead) {
+    auto block = [&](int tb, auto whole) {  // steps [tb, tb + kConvAhead), or up to te
+        constexpr bool kWhole = decltype(whole)::value;
         E in[kConvAhead];
         const E *px = x + (long long)tb * c.x_time;
+        E *py = y + (size_t)tb * c.dim;
 #pragma unroll
         for (int j = 0; j < kConvAhead; ++j) {
             in[j] = px[lo];
-            if (tb + j + 1 < te) px += c.x_time;
+            if (kWhole || tb + j + 1 < te) px += c.x_time;
         }
 #pragma unroll
         for (int j = 0; j < kConvAhead; ++j) {
-            if (tb + j >= te) break;
+            if (!kWhole && tb + j >= te) break;
 #pragma unroll
             for (int k = 0; k < W - 1; ++k) win[k] = win[k + 1];
             win[W - 1] = DT::to_float(in[j]);
             float p = bias;
 #pragma unroll
             for (int k = 0; k < W; ++k) p = fma_(w[k], win[k], p);
-            (y + (size_t)(tb + j) * c.dim)[lo] = DT::from_float(c.silu ? p * sigmoid_(p) : p);
+            py[lo] = DT::from_float(SILU ? p * sigmoid_(p) : p);
+            py += c.dim;
         }
-    }
+    };
+    int tb = t0;
+    for (; tb + kConvAhead <= te; tb += kConvAhead) block(tb, Index<1>());
+    if (tb < te) block(tb, Index<0>());
     for (int t = te; t < t1; ++t) (y + (size_t)t * c.dim)[lo] = DT::from_float(0.f);
     if (run == 0 && c.final_state) {
         float fin[W - 1];  // (all read before any is written: final_state may be the buffer of initial_state)
@@ -910,10 +917,12 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_forward_kernel(const r
 }
 
 // dxe[e] = sum_k w[k] gp[e - k] + grad_final, dw[k] = sum_t gp[t] xe[t + k], db = sum gp, with gp = grad_y silu'(p):
-// p is formed again from the W rows that the window holds: 42 us at that shape (111 MB at 2.6 TB/s; the vector units are
-// busy about half the time).  Runs of 128 steps leave too few waves (57 us), of 32 more ends to repeat (44 us); fetching the next
-// block's rows meanwhile costs registers, so waves (56 us).  partial: [workgroups of one channel group][W + 1][dim].
-template <typename DT, int W>
+// p is formed again from the W rows that the window holds: 27 us at that shape (111 MB at 4.1 TB/s).  Every step that waits for its
+// own load, or whose row is zero anyway, costs as much as a block: steps past the end left out 43 -> 29.5 us, the last steps of a run
+// loaded together 29.5 -> 27.  Runs of 128 steps leave too few waves (33 us), of 32 more ends to repeat (28 us); fetching the next
+// block's rows meanwhile, or a second copy of the block for a run's first rows, costs registers, so waves (48 against 42 us
+// then).  partial: [workgroups of one channel group][W + 1][dim].
+template <typename DT, int W, bool SILU>
 __global__ __launch_bounds__(kConvWaves *kWave) void conv_backward_kernel(const rnntConv c, int runs, int groups, float *partial) {
     typedef typename DT::elem E;
     __shared__ float s_sum[kConvWaves][W + 1][kWave];
@@ -929,7 +938,7 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_backward_kernel(const 
     float dw[W], db = 0.f;
 #pragma unroll
     for (int k = 0; k < W; ++k) dw[k] = 0.f;
-    if (b < c.batch) {
+    if (b < c.batch && ok) {
         const int len = clamp_len(c.lengths, (int)b, c.length);
         const int t0 = run * kRunBackward, t1 = t0 + kRunBackward < c.length ? t0 + kRunBackward : c.length;
         float w[W], win[W], gp[W];
@@ -943,10 +952,10 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_backward_kernel(const 
         const E *x = static_cast<const E *>(c.x) + b * c.x_batch;
         const E *gy = static_cast<const E *>(c.grad_y) + b * c.grad_y_batch;
         E *dx = static_cast<E *>(c.grad_x) + (size_t)b * c.length * c.dim;
-        E *di = c.grad_initial ? static_cast<E *>(c.grad_initial) + (size_t)b * (W - 1) * c.dim + d : nullptr;
+        E *di = c.grad_initial ? static_cast<E *>(c.grad_initial) + (size_t)b * (W - 1) * c.dim : nullptr;
         const E *gf = c.grad_final ? static_cast<const E *>(c.grad_final) + (size_t)b * (W - 1) * c.dim + d : nullptr;
         // Step s is newest in the window, gp[k] belongs to step s - (W - 1) + k; row t = s - (W - 1) of dx is then complete.
-        auto step = [&](int s, float xs, float gs, bool own) {
+        auto step = [&](float xs, float gs, bool own) {
 #pragma unroll
             for (int k = 0; k < W - 1; ++k) {
                 win[k] = win[k + 1];
@@ -957,7 +966,7 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_backward_kernel(const 
 #pragma unroll
             for (int k = 0; k < W; ++k) p = fma_(w[k], win[k], p);
             float v = gs;
-            if (c.silu) {
+            if (SILU) {
                 const float sg = sigmoid_(p);
                 v *= fma_(p * sg, 1.f - sg, sg);
             }
@@ -974,27 +983,30 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_backward_kernel(const 
             for (int k = 0; k < W; ++k) v = fma_(w[W - 1 - k], gp[k], v);
             return v;
         };
-        auto finish = [&](int t) {  // row t of dx, or of the initial state's gradient; any t
+        auto finish = [&](int t) {  // row t < len of dx, or of the initial state's gradient
             float v = gradient();
-            if (gf && t >= len - (W - 1) && t < len) v += DT::to_float(gf[(size_t)(t - (len - (W - 1))) * c.dim]);
-            if (!ok) return;
+            if (gf && t >= len - (W - 1)) v += DT::to_float(gf[(size_t)(t - (len - (W - 1))) * c.dim]);
             if (t >= 0)
-                (dx + (size_t)t * c.dim)[lo] = DT::from_float(t < len ? v : 0.f);
+                (dx + (size_t)t * c.dim)[lo] = DT::from_float(v);
             else if (di)
-                di[(size_t)(t + W - 1) * c.dim] = DT::from_float(v);
+                (di + (size_t)(t + W - 1) * c.dim)[lo] = DT::from_float(v);
         };
         // rows of dxe that this run writes: its own steps' x rows t0 .. t1-1 and, run 0, the W - 1 rows of the initial state
         const int first = run == 0 ? -(W - 1) : t0;
+        // (rows past the sequence's end are zero, and steps past it give nothing to any row)
+        const int end = len < t1 ? len : t1;
         if (first < len) {
 #pragma unroll
             for (int k = 0; k < W - 1; ++k)
                 win[k + 1] = first - (W - 1) + k >= -(W - 1) ? conv_in<DT, W>(c, (int)b, (long long)first - (W - 1) + k, d) : 0.f;
-        }
-        int s = first;
-        const int stop = t1 + W - 1;
-        while (s < stop) {
-            // whole blocks of the sequence and the run (no part of the final state: t < len - (W - 1)): loads first, no tests
-            if (s >= 0 && s + kConvAhead <= t1 && s + kConvAhead <= len) {
+            int s = first;
+            for (; s < 0; ++s) {  // the initial state's rows enter the window
+                step(conv_in<DT, W>(c, (int)b, s, d), 0.f, false);
+                gp[W - 1] = 0.f;  // (0 times an infinite derivative)
+            }
+            // Whole blocks of the sequence and the run (no part of the final state: t < len - (W - 1)): loads first, no tests.  The
+            // first begins with rows of the initial state, or of the run before, which are put where row t0 comes next.
+            for (; s + kConvAhead <= end; s += kConvAhead) {
                 E xin[kConvAhead], gin[kConvAhead];
                 const E *px = x + (long long)s * c.x_time, *pg = gy + (long long)s * c.grad_y_time;
 #pragma unroll
@@ -1004,29 +1016,39 @@ __global__ __launch_bounds__(kConvWaves *kWave) void conv_backward_kernel(const 
                     px += c.x_time;
                     pg += c.grad_y_time;
                 }
-                const int t = s - (W - 1);
-                E *pd = dx + (long long)t * c.dim;
+                E *pd = dx + (long long)(s - (W - 1)) * c.dim;
+                E *begins = run == 0 && di ? di : dx + (long long)t0 * c.dim;
+                const long long begins_row = run == 0 && di ? c.dim : 0;
 #pragma unroll
                 for (int j = 0; j < kConvAhead; ++j) {
-                    step(s + j, DT::to_float(xin[j]), DT::to_float(gin[j]), true);
-                    const float v = gradient();
-                    if (j >= W - 1 || t + j >= t0) {
-                        if (ok) pd[lo] = DT::from_float(v);
-                    } else if (t + j < 0 && di && ok) {
-                        di[(size_t)(t + j + W - 1) * c.dim] = DT::from_float(v);
-                    }
+                    step(DT::to_float(xin[j]), DT::to_float(gin[j]), true);
+                    E *p = j < W - 1 && s == t0 ? begins : pd;
+                    p[lo] = DT::from_float(gradient());
                     pd += c.dim;
+                    begins += begins_row;
                 }
-                s += kConvAhead;
-                continue;
             }
-            const bool live = s >= 0 && s < len;
-            step(s, s < len ? conv_in<DT, W>(c, (int)b, s, d) : 0.f, live ? DT::to_float((gy + (long long)s * c.grad_y_time)[lo]) : 0.f,
-                 live && s < t1);
-            if (!live) gp[W - 1] = 0.f;  // (0 times an infinite derivative)
-            if (s - (W - 1) >= first) finish(s - (W - 1));
-            ++s;
+            // what is left, and the W - 1 steps of the next run that these rows take part in
+            const int stop = end + W - 1;
+            for (; s < stop; s += kConvAhead) {
+                E xin[kConvAhead], gin[kConvAhead];
+#pragma unroll
+                for (int j = 0; j < kConvAhead; ++j) {
+                    const long long row = s + j < len ? s + j : (len > 0 ? len - 1 : 0);
+                    xin[j] = (x + row * c.x_time)[lo];
+                    gin[j] = (gy + row * c.grad_y_time)[lo];
+                }
+#pragma unroll
+                for (int j = 0; j < kConvAhead; ++j) {
+                    if (s + j >= stop) break;
+                    const bool live = s + j < len;
+                    step(live ? DT::to_float(xin[j]) : 0.f, live ? DT::to_float(gin[j]) : 0.f, live && s + j < t1);
+                    if (!live) gp[W - 1] = 0.f;
+                    if (s + j - (W - 1) >= first) finish(s + j - (W - 1));
+                }
+            }
         }
+        for (int t = len > t0 ? len : t0; t < t1; ++t) (dx + (size_t)t * c.dim)[lo] = DT::from_float(0.f);
     }
 #pragma unroll
     for (int k = 0; k < W; ++k) s_sum[wave][k][lane] = dw[k];
@@ -1252,7 +1274,7 @@ inline bool conv_shape_ok(int batch, int length, int dim, int width) {
 template <typename DT, int W>
 rnntStatus_t conv_forward(const rnntConv &c, hipStream_t st) {
     const unsigned grid = (unsigned)(conv_items(c.batch, c.length, kRunForward) * groups_of(c.dim));
-    hipLaunchKernelGGL((conv_forward_kernel<DT, W>), dim3(grid), dim3(kConvWaves * kWave), 0, st, c, runs_of(c.length, kRunForward),
+    hipLaunchKernelGGL((c.silu ? conv_forward_kernel<DT, W, true> : conv_forward_kernel<DT, W, false>), dim3(grid), dim3(kConvWaves * kWave), 0, st, c, runs_of(c.length, kRunForward),
                        groups_of(c.dim));
     return launched();
 }
@@ -1260,7 +1282,7 @@ template <typename DT, int W>
 rnntStatus_t conv_backward(const rnntConv &c, hipStream_t st) {
     const int parts = (int)conv_items(c.batch, c.length, kRunBackward);
     float *partial = static_cast<float *>(c.workspace);
-    hipLaunchKernelGGL((conv_backward_kernel<DT, W>), dim3((unsigned)((long long)parts * groups_of(c.dim))), dim3(kConvWaves * kWave), 0,
+    hipLaunchKernelGGL((c.silu ? conv_backward_kernel<DT, W, true> : conv_backward_kernel<DT, W, false>), dim3((unsigned)((long long)parts * groups_of(c.dim))), dim3(kConvWaves * kWave), 0,
                        st, c, runs_of(c.length, kRunBackward), groups_of(c.dim), partial);
     hipLaunchKernelGGL((conv_backward_sum_kernel<W>), dim3((unsigned)(((long long)(W + 1) * c.dim + kWave - 1) / kWave)), dim3(1024), 0,
                        st, c, static_cast<const float *>(partial), parts);
