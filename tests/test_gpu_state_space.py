@@ -16,8 +16,8 @@ U = plain.U
 
 
 def lens_for(kind, B, L):
-    if kind is None:
-        return None
+    if kind is None or torch.is_tensor(kind):
+        return kind
     some = [L, 0, 1, max(1, L // 2), max(1, L - 1), (L + 2) // 3]
     return torch.tensor([some[i % len(some)] for i in range(B)], dtype=torch.int32)
 
@@ -271,6 +271,14 @@ def test_conv_against_plain(dtype, W, B, L, D):
 @pytest.mark.parametrize("bias", [True, False])
 def test_conv_options(silu, state, bias):
     check_conv(6, 20, 40, 4, torch.float32, True, silu, state, bias)
+
+
+@pytest.mark.parametrize("W", [2, 3, 4])
+@pytest.mark.parametrize("state", [True, False])
+def test_conv_ends_around_blocks_and_runs(W, state):
+    """Sequences that end in, before and behind blocks of 8 steps and runs of 32 and 64, at every distance up to the filter's width."""
+    lens = torch.tensor([*range(13), *range(28, 37), *range(60, 76), *range(124, 141)], dtype=torch.int32)
+    check_conv(len(lens), 140, 5, W, torch.float32, lens, state=state, seed=W)
 
 
 def test_conv_layouts():
