@@ -419,7 +419,8 @@ rnntStatus_t rnnt_process_logits(const void *x, int rows, int V, rnntDtype_t dty
 
 /*
  * ---- the prediction network's layers ------------------------------------------------------------------------------
- * The reference's prediction network is embedding -> LSTM -> Linear (src/decoder/decoder.py:5-44).
+ * The reference's prediction network is embedding -> LSTM -> Linear (src/decoder/decoder.py:5-44).  Sizes that would need 2^32
+ * threads or more in one launch give RNNT_STATUS_INVALID_VALUE from every call, the size functions among them.
  *
  * Token embedding (src/decoder/decoder.py:9): out[i, :] = scale * weight[tokens[i], :], rounded once; tokens are int32 or int64
  * (tokens_64 = 1), weight rows weight_stride elements apart, out [n, dim] contiguous.  A token outside [0, vocab) gives a
