@@ -78,8 +78,10 @@ bool wants_grad(std::initializer_list<const Tensor *> inputs) {
 }
 
 // A call that a graph captures, on a leaf that an eager graph made on the default stream still holds: the backward pass would
-// wait for the default stream inside the capture, which ends the process rather than raising.
+// wait for the default stream inside the capture, which ends the process rather than raising.  `inputs` are the caller's own
+// tensors, before any is laid out: the copy of a leaf is no leaf.
 void check_capture(std::initializer_list<const Tensor *> inputs, const char *op) {
+    if (!at::GradMode::is_enabled()) return;
     for (const Tensor *t : inputs) {
         if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
         const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
@@ -166,12 +168,12 @@ Tensor token_embedding_op(const Tensor &tokens_in, const Tensor &weight_in, doub
                       "too many tokens (at most 2^30), or too large a weight (2^26 rows, 2^21 columns) for one call");
     check_on_device(weight_in, "token_embedding");
     check_same_device(tokens_in, weight_in, "tokens");
+    check_capture({&weight_in}, "token_embedding");
     const Tensor tokens = tokens_in.contiguous();
     const Tensor weight = weight_in.size(1) == 1 || weight_in.stride(1) == 1 ? weight_in : weight_in.contiguous();
     const bool ordered = weight.size(0) == 1 || weight.stride(0) >= weight.size(1);  // (an expanded weight is laid out first)
     const Tensor w = ordered ? weight : weight.contiguous();
     if (!wants_grad({&w})) return embed_forward(tokens, w, scale);
-    check_capture({&weight_in}, "token_embedding");
     return EmbedFunction::apply(tokens, w, scale, padding);
 }
 
@@ -276,11 +278,11 @@ std::tuple<Tensor, Tensor> causal_conv_op(const Tensor &x_in, const Tensor &weig
     check_same_device(bias, x_in, "bias");
     check_same_device(initial, x_in, "initial_state");
     check_same_device(lengths, x_in, "lengths");
+    check_capture({&x_in, &weight_in, &bias, &initial}, "causal_conv");
     const Tensor x = rows_of(x_in), weight = weight_in.contiguous();
     if (bias.defined()) bias = bias.contiguous();
     if (initial.defined()) initial = initial.contiguous();
     if (!wants_grad({&x, &weight, &bias, &initial})) return conv_forward(x, weight, bias, initial, lengths, silu);
-    check_capture({&x_in, &weight_in, &bias, &initial}, "causal_conv");
     const auto out = ConvFunction::apply(x, weight, bias.defined() ? MaybeTensor(bias) : MaybeTensor(),
                                          initial.defined() ? MaybeTensor(initial) : MaybeTensor(), lengths_in, silu);
     return {out[0], out[1]};
@@ -487,6 +489,7 @@ ScanIn scan_check(const Tensor &x, const Tensor &dt, const Tensor &A, const Tens
     const Tensor *all[] = {&dt, &A, &B, &C, &in.D, &in.z, &in.dt_bias, &in.initial, &in.lengths};
     const char *names[] = {"dt", "A", "B", "C", "D", "z", "dt_bias", step ? "state" : "initial_state", "lengths"};
     for (int i = 0; i < 9; ++i) check_same_device(*all[i], x, names[i]);
+    if (!step) check_capture({&x, &dt, &A, &B, &C, &in.D, &in.z, &in.dt_bias, &in.initial}, op);
     in.x = rows_of(x);
     in.dt = rows_of(dt);
     in.B = rows_of(B);
@@ -507,7 +510,6 @@ std::tuple<Tensor, Tensor> selective_scan_op(const Tensor &x, const Tensor &dt, 
         auto out = scan_forward(in, false);
         return {std::get<0>(out), std::get<1>(out)};
     }
-    check_capture({&in.x, &in.dt, &in.A, &in.B, &in.C, &in.D, &in.z, &in.dt_bias, &in.initial}, "selective_scan");
     auto maybe = [](const Tensor &t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); };
     const auto out = ScanFunction::apply(in.x, in.dt, in.A, in.B, in.C, maybe(in.D), maybe(in.z), maybe(in.dt_bias), maybe(in.initial),
                                          maybe(in.lengths));

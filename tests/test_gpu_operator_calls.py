@@ -1,0 +1,42 @@
+"""GPU tests of how the prediction network's and the decoder's operators may be called: captured calls on leaves that the call
+has to lay out."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+def apart(*shape):
+    """A leaf whose elements are not adjacent, so that the call makes a copy of it."""
+    t = torch.randn(*shape, 2, generator=torch.Generator().manual_seed(7)).to(DEV)
+    return t[..., 0].requires_grad_(True)
+
+
+def scan_args():
+    r = lambda *s: torch.randn(*s, generator=torch.Generator().manual_seed(8)).to(DEV)  # noqa: E731
+    return dict(x=r(2, 5, 64), dt=r(2, 5, 64), A=-r(64, 8).abs(), B=r(2, 5, 8), C=r(2, 5, 8), D=r(64), z=r(2, 5, 64), dt_bias=r(64),
+                initial_state=r(2, 64, 8))
+
+
+def conv_args():
+    r = lambda *s: torch.randn(*s, generator=torch.Generator().manual_seed(9)).to(DEV)  # noqa: E731
+    return dict(x=r(2, 5, 64), weight=r(64, 4), bias=r(64), initial_state=r(2, 3, 64))
+
+
+@pytest.mark.parametrize("op,name", [("selective_scan", n) for n in ("x", "dt", "A", "B", "C", "D", "z", "dt_bias", "initial_state")] +
+                         [("causal_conv", n) for n in ("x", "weight", "bias", "initial_state")])
+def test_capture_is_refused_for_a_leaf_that_the_call_lays_out(op, name):
+    """Refused before anything is launched, as for a leaf that the call takes as it is."""
+    import rnnt_amd
+
+    args = scan_args() if op == "selective_scan" else conv_args()
+    args[name] = apart(*args[name].shape)
+    assert args[name].is_leaf and not args[name].is_contiguous()
+    held = getattr(rnnt_amd, op)(**args)
+    graph, scratch = torch.cuda.CUDAGraph(), torch.zeros(1, device=DEV)
+    with torch.cuda.graph(graph):
+        scratch.add_(1)
+        with pytest.raises(RuntimeError, match="cannot be captured while"):
+            getattr(rnnt_amd, op)(**args)
+    del held
