@@ -77,6 +77,13 @@ bool wants_grad(std::initializer_list<const Tensor *> inputs) {
     return false;
 }
 
+// There are no forward-mode derivatives here.  An input with a tangent need not require grad, and then no autograd function would
+// refuse it: the tangent would be lost without an error.
+void check_tangents(std::initializer_list<const Tensor *> inputs, const char *op) {
+    for (const Tensor *t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), "rnnt_amd.", op, " has no forward-mode derivative");
+}
+
 // A call that a graph captures, on a leaf that an eager graph made on the default stream still holds: the backward pass would
 // wait for the default stream inside the capture, which ends the process rather than raising.  `inputs` are the caller's own
 // tensors, before any is laid out: the copy of a leaf is no leaf.
@@ -166,6 +173,7 @@ Tensor token_embedding_op(const Tensor &tokens_in, const Tensor &weight_in, doub
                           rnnt_token_embedding_workspace_size(tokens_in.numel(), (int)weight_in.size(0), (int)weight_in.size(1), &need) ==
                               RNNT_STATUS_SUCCESS,
                       "too many tokens (at most 2^30), or too large a weight (2^26 rows, 2^21 columns) for one call");
+    check_tangents({&weight_in}, "token_embedding");
     check_on_device(weight_in, "token_embedding");
     check_same_device(tokens_in, weight_in, "tokens");
     check_capture({&weight_in}, "token_embedding");
@@ -273,6 +281,7 @@ std::tuple<Tensor, Tensor> causal_conv_op(const Tensor &x_in, const Tensor &weig
                           rnnt_causal_conv_workspace_size((int)x_in.size(0), (int)x_in.size(1), (int)x_in.size(2),
                                                           (int)weight_in.size(1), &need) == RNNT_STATUS_SUCCESS,
                       "x is too large for one call");
+    check_tangents({&x_in, &weight_in, &bias, &initial}, "causal_conv");
     check_on_device(x_in, "causal_conv");
     check_same_device(weight_in, x_in, "weight");
     check_same_device(bias, x_in, "bias");
@@ -333,6 +342,7 @@ std::tuple<Tensor, Tensor> causal_conv_step_op(const Tensor &x_in, const Tensor 
     check_conv_weights(weight_in, bias, x_in.size(1));
     check_conv_state(state_in, x_in, weight_in.size(1), "state");
     TORCH_CHECK_VALUE(x_in.numel() < (1ll << 31) && x_in.size(1) < (1ll << 28), "x is too large for one call");
+    check_tangents({&x_in, &state_in, &weight_in, &bias}, "causal_conv_step");
     check_on_device(x_in, "causal_conv_step");
     check_same_device(state_in, x_in, "state");
     check_same_device(weight_in, x_in, "weight");
@@ -485,6 +495,7 @@ ScanIn scan_check(const Tensor &x, const Tensor &dt, const Tensor &A, const Tens
                           rnnt_selective_scan_states_size((int)x.size(0), step ? 1 : (int)x.size(1), (int)x.size(-1), (int)A.size(1),
                                                           &need) == RNNT_STATUS_SUCCESS,
                       "x is too large for one call");
+    check_tangents({&x, &dt, &A, &B, &C, &in.D, &in.z, &in.dt_bias, &in.initial}, op);
     check_on_device(x, op);
     const Tensor *all[] = {&dt, &A, &B, &C, &in.D, &in.z, &in.dt_bias, &in.initial, &in.lengths};
     const char *names[] = {"dt", "A", "B", "C", "D", "z", "dt_bias", step ? "state" : "initial_state", "lengths"};
@@ -539,7 +550,8 @@ struct RulesIn {
 };
 
 RulesIn rules_check(const Tensor &x, const MaybeTensor &bias_in, const MaybeTensor &allowed_in, const MaybeTensor &history_in,
-                    const MaybeTensor &history_lens_in, double repetition, double presence, double frequency, const char *op) {
+                    const MaybeTensor &history_lens_in, double repetition, double presence, double frequency, bool values,
+                    const char *op) {
     RulesIn in = {x, given(bias_in), given(allowed_in), given(history_in), given(history_lens_in)};
     TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) >= 1 && x.size(1) >= 1, "x must be a non-empty [rows, V] tensor");
     dtype_code(x, "x");
@@ -583,6 +595,7 @@ RulesIn rules_check(const Tensor &x, const MaybeTensor &bias_in, const MaybeTens
     TORCH_CHECK_VALUE((float)repetition > 0.f && std::isfinite((float)repetition), "repetition_penalty must be positive and finite");
     TORCH_CHECK_VALUE(std::isfinite((float)presence) && std::isfinite((float)frequency),
                       "presence_penalty and frequency_penalty must be finite");
+    if (values) check_tangents({&x, &in.bias}, op);  // (a token alone has no derivative)
     check_on_device(x, op);
     check_same_device(in.bias, x, "bias");
     check_same_device(in.allowed, x, "allowed");
@@ -611,7 +624,7 @@ RulesIn rules_check(const Tensor &x, const MaybeTensor &bias_in, const MaybeTens
 std::tuple<Tensor, Tensor> row_rules_op(const Tensor &x, const MaybeTensor &bias, const MaybeTensor &allowed, const MaybeTensor &history,
                                         const MaybeTensor &history_lens, double repetition, double presence, double frequency,
                                         bool want_logp) {
-    const RulesIn in = rules_check(x, bias, allowed, history, history_lens, repetition, presence, frequency,
+    const RulesIn in = rules_check(x, bias, allowed, history, history_lens, repetition, presence, frequency, want_logp,
                                    want_logp ? "row_max_logp" : "row_argmax");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     Tensor token = at::empty({in.rows}, x.options().dtype(at::kInt));
@@ -628,7 +641,7 @@ std::tuple<Tensor, Tensor> row_rules_op(const Tensor &x, const MaybeTensor &bias
 Tensor process_logits_op(const Tensor &x, const MaybeTensor &bias, const MaybeTensor &allowed, const MaybeTensor &history,
                          const MaybeTensor &history_lens, double repetition, double presence, double frequency,
                          const MaybeTensor &out_in) {
-    const RulesIn in = rules_check(x, bias, allowed, history, history_lens, repetition, presence, frequency, "process_logits");
+    const RulesIn in = rules_check(x, bias, allowed, history, history_lens, repetition, presence, frequency, true, "process_logits");
     check_no_grad({&x, &in.bias}, "process_logits");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     Tensor out;

@@ -1,7 +1,8 @@
 """GPU tests of how the prediction network's and the decoder's operators may be called: captured calls on leaves that the call
-has to lay out."""
+has to lay out, forward-mode derivatives."""
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -40,3 +41,20 @@ def test_capture_is_refused_for_a_leaf_that_the_call_lays_out(op, name):
         with pytest.raises(RuntimeError, match="cannot be captured while"):
             getattr(rnnt_amd, op)(**args)
     del held
+
+
+def test_a_tangent_is_refused_on_the_device():
+    import rnnt_amd
+
+    for op, args in (("selective_scan", scan_args()), ("causal_conv", conv_args())):
+        for name in args:
+            with fwAD.dual_level():
+                dual = fwAD.make_dual(args[name], torch.ones_like(args[name]))
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    getattr(rnnt_amd, op)(**{**args, name: dual})
+            getattr(rnnt_amd, op)(**args)
+    net = rnnt_amd.PredictionNet(12, 8, 8).to(DEV)
+    name, weight = "embedding.weight", net.embedding.weight
+    with fwAD.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.functional_call(net, {name: fwAD.make_dual(weight.detach(), torch.ones_like(weight))},
+                                   (torch.zeros(1, 2, dtype=torch.int32, device=DEV),))

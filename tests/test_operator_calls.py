@@ -1,0 +1,47 @@
+"""CPU tests of how the prediction network's and the decoder's operators may be called.  Nothing is launched."""
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+import rnnt_amd
+
+R = rnnt_amd.LogitRules
+
+
+def calls():
+    """name -> (call of keyword tensors, the tensors)."""
+    r = lambda *s: torch.randn(*s, generator=torch.Generator().manual_seed(3))  # noqa: E731
+    scan = dict(x=r(2, 5, 6), dt=r(2, 5, 6), A=-r(6, 8).abs(), B=r(2, 5, 8), C=r(2, 5, 8), D=r(6), z=r(2, 5, 6), dt_bias=r(6),
+                initial_state=r(2, 6, 8))
+    step = {k: v[:, 0] if k in ("x", "dt", "B", "C", "z") else v for k, v in scan.items() if k != "initial_state"}
+    rules = dict(x=r(4, 9), bias=r(9))
+    return {
+        "token_embedding": (lambda weight: rnnt_amd.token_embedding(torch.zeros(3, dtype=torch.int32), weight), dict(weight=r(5, 4))),
+        "causal_conv": (rnnt_amd.causal_conv, dict(x=r(2, 5, 6), weight=r(6, 4), bias=r(6), initial_state=r(2, 3, 6))),
+        "causal_conv_step": (rnnt_amd.causal_conv_step, dict(x=r(2, 6), state=r(2, 3, 6), weight=r(6, 4), bias=r(6))),
+        "selective_scan": (rnnt_amd.selective_scan, scan),
+        "selective_scan_step": (rnnt_amd.selective_scan_step, {**step, "state": r(2, 6, 8)}),
+        "row_max_logp": (lambda x, bias: rnnt_amd.row_max_logp(x, R(bias=bias)), rules),
+        "process_logits": (lambda x, bias: rnnt_amd.process_logits(x, R(bias=bias)), rules),
+        "row_argmax": (lambda x, bias: rnnt_amd.row_argmax(x, R(bias=bias)), rules),
+    }
+
+
+@pytest.mark.parametrize("op,name", [(op, k) for op, (_, t) in calls().items() for k in t])
+def test_a_tangent_is_refused_and_not_lost(op, name):
+    """Whether or not the input requires grad, and without grad mode too (which leaves forward derivatives on); a token alone has no
+    derivative, so that row_argmax goes on to the next check."""
+    call, tensors = calls()[op]
+    for requires_grad in (False, True):
+        for mode in (torch.enable_grad(), torch.no_grad()):
+            with fwAD.dual_level(), mode:
+                leaf = tensors[name].clone().requires_grad_(requires_grad)
+                dual = fwAD.make_dual(leaf, torch.ones_like(leaf))
+                if op == "row_argmax":
+                    with pytest.raises(RuntimeError, match="no CPU path"):
+                        call(**{**tensors, name: dual})
+                    continue
+                with pytest.raises(NotImplementedError, match=op + " has no forward-mode derivative"):
+                    call(**{**tensors, name: dual})
+    with pytest.raises(RuntimeError, match="no CPU path"):       # outside of a level, nothing is refused for it
+        call(**tensors)
