@@ -664,22 +664,23 @@ Tensor process_logits_op(const Tensor &x, const MaybeTensor &bias, const MaybeTe
 
 }  // namespace
 
+// (a caller's result buffer is declared as written: a compiled graph would drop a call whose returned tensors it does not use)
 TORCH_LIBRARY_FRAGMENT(rnnt_amd, m) {
     m.def("token_embedding(Tensor tokens, Tensor weight, float scale, int padding_idx) -> Tensor", &token_embedding_op);
     m.def("causal_conv(Tensor x, Tensor weight, Tensor? bias, Tensor? initial_state, Tensor? lengths, bool silu) -> (Tensor, Tensor)",
           &causal_conv_op);
-    m.def("causal_conv_step(Tensor x, Tensor state, Tensor weight, Tensor? bias, bool silu, Tensor? state_out) -> (Tensor, Tensor)",
+    m.def("causal_conv_step(Tensor x, Tensor state, Tensor weight, Tensor? bias, bool silu, Tensor(a!)? state_out) -> (Tensor, Tensor(a!))",
           &causal_conv_step_op);
     m.def("selective_scan(Tensor x, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor? D, Tensor? z, Tensor? dt_bias, "
           "Tensor? initial_state, Tensor? lengths) -> (Tensor, Tensor)",
           &selective_scan_op);
     m.def("selective_scan_step(Tensor x, Tensor dt, Tensor A, Tensor B, Tensor C, Tensor state, Tensor? D, Tensor? z, "
-          "Tensor? dt_bias, Tensor? state_out) -> (Tensor, Tensor)",
+          "Tensor? dt_bias, Tensor(a!)? state_out) -> (Tensor, Tensor(a!))",
           &selective_scan_step_op);
     m.def("row_rules(Tensor x, Tensor? bias, Tensor? allowed, Tensor? history, Tensor? history_lens, float repetition_penalty, "
           "float presence_penalty, float frequency_penalty, bool want_logp) -> (Tensor, Tensor)",
           &row_rules_op);
     m.def("process_logits(Tensor x, Tensor? bias, Tensor? allowed, Tensor? history, Tensor? history_lens, float repetition_penalty, "
-          "float presence_penalty, float frequency_penalty, Tensor? out) -> Tensor",
+          "float presence_penalty, float frequency_penalty, Tensor(a!)? out) -> Tensor(a!)",
           &process_logits_op);
 }

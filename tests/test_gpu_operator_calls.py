@@ -1,8 +1,10 @@
 """GPU tests of how the prediction network's and the decoder's operators may be called: captured calls on leaves that the call
-has to lay out, forward-mode derivatives."""
+has to lay out, forward-mode derivatives, results that a compiled graph uses only through the caller's buffer."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
+
+from test_operator_calls import writers
 
 pytestmark = pytest.mark.gpu
 DEV = torch.device("cuda:0")
@@ -58,3 +60,20 @@ def test_a_tangent_is_refused_on_the_device():
     with fwAD.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
         torch.func.functional_call(net, {name: fwAD.make_dual(weight.detach(), torch.ones_like(weight))},
                                    (torch.zeros(1, 2, dtype=torch.int32, device=DEV),))
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+@pytest.mark.parametrize("fn,args,op", writers(), ids=lambda v: v if isinstance(v, str) else "")
+def test_a_compiled_graph_writes_the_callers_buffer(fn, args, op):
+    from rnnt_amd import _torch_binding
+
+    _torch_binding.load()
+    args = [t.to(DEV) for t in args]
+    want = fn(*args[:-1], torch.zeros_like(args[-1]))
+    assert torch.count_nonzero(want)
+    out = torch.zeros_like(want)
+    for graph in (torch.jit.script(fn), torch.jit.trace(fn, (*args[:-1], torch.zeros_like(want)), check_trace=False)):
+        out.zero_()
+        for _ in range(3):      # (the first runs of a compiled graph record it, the later ones are optimised)
+            graph(*args[:-1], out)
+        assert torch.equal(out, want)

@@ -45,3 +45,51 @@ def test_a_tangent_is_refused_and_not_lost(op, name):
                     call(**{**tensors, name: dual})
     with pytest.raises(RuntimeError, match="no CPU path"):       # outside of a level, nothing is refused for it
         call(**tensors)
+
+
+def write_logits(x: torch.Tensor, out: torch.Tensor):
+    torch.ops.rnnt_amd.process_logits(x, None, None, None, None, 1.0, 0.0, 0.0, out)
+    return out
+
+
+def write_conv(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, out: torch.Tensor):
+    torch.ops.rnnt_amd.causal_conv_step(x, state, weight, None, True, out)
+    return out
+
+
+def write_scan(x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, state: torch.Tensor, out: torch.Tensor):
+    torch.ops.rnnt_amd.selective_scan_step(x, x, A, B, B, state, None, None, None, out)
+    return out
+
+
+def writers():
+    """(function that writes the last of its tensors and uses nothing that the call returns, its tensors, name of the operator)"""
+    r = lambda *s: torch.randn(*s, generator=torch.Generator().manual_seed(5))  # noqa: E731
+    return [(write_logits, [r(3, 9), torch.zeros(3, 9)], "process_logits"),
+            (write_conv, [r(2, 6), r(2, 3, 6), r(6, 4), torch.zeros(2, 3, 6)], "causal_conv_step"),
+            (write_scan, [r(2, 6), -r(6, 8).abs(), r(2, 8), r(2, 6, 8), torch.zeros(2, 6, 8)], "selective_scan_step")]
+
+
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+@pytest.mark.parametrize("fn,args,op", writers(), ids=lambda v: v if isinstance(v, str) else "")
+def test_a_compiled_graph_keeps_a_call_for_the_buffer_it_writes(fn, args, op):
+    from rnnt_amd import _torch_binding
+
+    schema = getattr(_torch_binding.load(), op).default._schema
+    assert schema.is_mutable
+    assert [a.name for a in schema.arguments if a.alias_info is not None and a.alias_info.is_write] == [
+        "out" if op == "process_logits" else "state_out"]
+    script = torch.jit.script(fn)
+    graph = script.graph.copy()
+    torch._C._jit_pass_dce(graph)
+    assert "rnnt_amd::" + op in str(graph)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        script(*args)
+
+
+def test_calls_that_write_no_buffer_say_so():
+    from rnnt_amd import _torch_binding
+
+    ops = _torch_binding.load()
+    for name in ("token_embedding", "causal_conv", "selective_scan", "row_rules"):
+        assert not getattr(ops, name).default._schema.is_mutable
