@@ -84,6 +84,13 @@ void check_tangents(std::initializer_list<const Tensor *> inputs, const char *op
         TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), "rnnt_amd.", op, " has no forward-mode derivative");
 }
 
+// Calls without any derivative.  `tensors`: what the call reads, and the buffer it writes: a buffer that autograd follows would keep the
+// history of the values that are gone.
+void check_no_grad(std::initializer_list<const Tensor *> tensors, const char *op) {
+    check_tangents(tensors, op);
+    TORCH_CHECK(!wants_grad(tensors), "rnnt_amd.", op, " is for decoding and has no backward: call it under torch.no_grad()");
+}
+
 // A call that a graph captures, on a leaf that an eager graph made on the default stream still holds: the backward pass would
 // wait for the default stream inside the capture, which ends the process rather than raising.  `inputs` are the caller's own
 // tensors, before any is laid out: the copy of a leaf is no leaf.
@@ -330,10 +337,6 @@ Tensor state_buffer(const MaybeTensor &out, const Tensor &state, std::initialize
     return *out;
 }
 
-void check_no_grad(std::initializer_list<const Tensor *> inputs, const char *op) {
-    TORCH_CHECK(!wants_grad(inputs), "rnnt_amd.", op, " is for decoding and has no backward: call it under torch.no_grad()");
-}
-
 std::tuple<Tensor, Tensor> causal_conv_step_op(const Tensor &x_in, const Tensor &state_in, const Tensor &weight_in,
                                                const MaybeTensor &bias_in, bool silu, const MaybeTensor &state_out) {
     dtype_code(x_in, "x");
@@ -342,12 +345,12 @@ std::tuple<Tensor, Tensor> causal_conv_step_op(const Tensor &x_in, const Tensor 
     check_conv_weights(weight_in, bias, x_in.size(1));
     check_conv_state(state_in, x_in, weight_in.size(1), "state");
     TORCH_CHECK_VALUE(x_in.numel() < (1ll << 31) && x_in.size(1) < (1ll << 28), "x is too large for one call");
-    check_tangents({&x_in, &state_in, &weight_in, &bias}, "causal_conv_step");
+    const Tensor written = given(state_out);
+    check_no_grad({&x_in, &state_in, &weight_in, &bias, &written}, "causal_conv_step");
     check_on_device(x_in, "causal_conv_step");
     check_same_device(state_in, x_in, "state");
     check_same_device(weight_in, x_in, "weight");
     check_same_device(bias, x_in, "bias");
-    check_no_grad({&x_in, &state_in, &weight_in, &bias}, "causal_conv_step");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x_in.device());
     Tensor out = state_buffer(state_out, state_in, {&x_in, &weight_in, &bias});
     const Tensor x = rows_of(x_in), state = state_in.contiguous(), weight = weight_in.contiguous();
@@ -466,7 +469,8 @@ public:
 };
 
 ScanIn scan_check(const Tensor &x, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const MaybeTensor &D,
-                  const MaybeTensor &z, const MaybeTensor &dt_bias, const Tensor &state, const MaybeTensor &lengths, bool step) {
+                  const MaybeTensor &z, const MaybeTensor &dt_bias, const Tensor &state, const MaybeTensor &lengths, bool step,
+                  const Tensor &written = Tensor()) {
     ScanIn in = {x, dt, A, B, C, given(D), given(z), given(dt_bias), state, given(lengths)};
     const char *op = step ? "selective_scan_step" : "selective_scan";
     dtype_code(x, "x");
@@ -495,7 +499,10 @@ ScanIn scan_check(const Tensor &x, const Tensor &dt, const Tensor &A, const Tens
                           rnnt_selective_scan_states_size((int)x.size(0), step ? 1 : (int)x.size(1), (int)x.size(-1), (int)A.size(1),
                                                           &need) == RNNT_STATUS_SUCCESS,
                       "x is too large for one call");
-    check_tangents({&x, &dt, &A, &B, &C, &in.D, &in.z, &in.dt_bias, &in.initial}, op);
+    if (step)
+        check_no_grad({&x, &dt, &A, &B, &C, &in.D, &in.z, &in.dt_bias, &in.initial, &written}, op);
+    else
+        check_tangents({&x, &dt, &A, &B, &C, &in.D, &in.z, &in.dt_bias, &in.initial}, op);
     check_on_device(x, op);
     const Tensor *all[] = {&dt, &A, &B, &C, &in.D, &in.z, &in.dt_bias, &in.initial, &in.lengths};
     const char *names[] = {"dt", "A", "B", "C", "D", "z", "dt_bias", step ? "state" : "initial_state", "lengths"};
@@ -530,8 +537,7 @@ std::tuple<Tensor, Tensor> selective_scan_op(const Tensor &x, const Tensor &dt, 
 std::tuple<Tensor, Tensor> selective_scan_step_op(const Tensor &x, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C,
                                                   const Tensor &state, const MaybeTensor &D, const MaybeTensor &z,
                                                   const MaybeTensor &dt_bias, const MaybeTensor &state_out) {
-    const ScanIn in = scan_check(x, dt, A, B, C, D, z, dt_bias, state, MaybeTensor(), true);
-    check_no_grad({&in.x, &in.dt, &in.A, &in.B, &in.C, &in.D, &in.z, &in.dt_bias, &in.initial}, "selective_scan_step");
+    const ScanIn in = scan_check(x, dt, A, B, C, D, z, dt_bias, state, MaybeTensor(), true, given(state_out));
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     Tensor out = state_buffer(state_out, state, {&x, &dt, &A, &B, &C, &in.D, &in.z, &in.dt_bias});
     Tensor y = at::empty(x.sizes(), x.options());
@@ -550,8 +556,8 @@ struct RulesIn {
 };
 
 RulesIn rules_check(const Tensor &x, const MaybeTensor &bias_in, const MaybeTensor &allowed_in, const MaybeTensor &history_in,
-                    const MaybeTensor &history_lens_in, double repetition, double presence, double frequency, bool values,
-                    const char *op) {
+                    const MaybeTensor &history_lens_in, double repetition, double presence, double frequency, const char *op,
+                    bool values, const Tensor &written = Tensor()) {
     RulesIn in = {x, given(bias_in), given(allowed_in), given(history_in), given(history_lens_in)};
     TORCH_CHECK_VALUE(x.dim() == 2 && x.size(0) >= 1 && x.size(1) >= 1, "x must be a non-empty [rows, V] tensor");
     dtype_code(x, "x");
@@ -596,6 +602,7 @@ RulesIn rules_check(const Tensor &x, const MaybeTensor &bias_in, const MaybeTens
     TORCH_CHECK_VALUE(std::isfinite((float)presence) && std::isfinite((float)frequency),
                       "presence_penalty and frequency_penalty must be finite");
     if (values) check_tangents({&x, &in.bias}, op);  // (a token alone has no derivative)
+    check_no_grad({&written}, op);
     check_on_device(x, op);
     check_same_device(in.bias, x, "bias");
     check_same_device(in.allowed, x, "allowed");
@@ -624,8 +631,8 @@ RulesIn rules_check(const Tensor &x, const MaybeTensor &bias_in, const MaybeTens
 std::tuple<Tensor, Tensor> row_rules_op(const Tensor &x, const MaybeTensor &bias, const MaybeTensor &allowed, const MaybeTensor &history,
                                         const MaybeTensor &history_lens, double repetition, double presence, double frequency,
                                         bool want_logp) {
-    const RulesIn in = rules_check(x, bias, allowed, history, history_lens, repetition, presence, frequency, want_logp,
-                                   want_logp ? "row_max_logp" : "row_argmax");
+    const RulesIn in = rules_check(x, bias, allowed, history, history_lens, repetition, presence, frequency,
+                                   want_logp ? "row_max_logp" : "row_argmax", want_logp);
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     Tensor token = at::empty({in.rows}, x.options().dtype(at::kInt));
     Tensor logp = at::empty({want_logp ? in.rows : 0}, x.options().dtype(at::kFloat));
@@ -641,7 +648,8 @@ std::tuple<Tensor, Tensor> row_rules_op(const Tensor &x, const MaybeTensor &bias
 Tensor process_logits_op(const Tensor &x, const MaybeTensor &bias, const MaybeTensor &allowed, const MaybeTensor &history,
                          const MaybeTensor &history_lens, double repetition, double presence, double frequency,
                          const MaybeTensor &out_in) {
-    const RulesIn in = rules_check(x, bias, allowed, history, history_lens, repetition, presence, frequency, true, "process_logits");
+    const RulesIn in = rules_check(x, bias, allowed, history, history_lens, repetition, presence, frequency, "process_logits", true,
+                                   given(out_in));
     check_no_grad({&x, &in.bias}, "process_logits");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     Tensor out;

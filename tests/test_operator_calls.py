@@ -93,3 +93,19 @@ def test_calls_that_write_no_buffer_say_so():
     ops = _torch_binding.load()
     for name in ("token_embedding", "causal_conv", "selective_scan", "row_rules"):
         assert not getattr(ops, name).default._schema.is_mutable
+
+
+@pytest.mark.parametrize("fn,args,op", writers(), ids=lambda v: v if isinstance(v, str) else "")
+def test_a_buffer_that_autograd_follows_is_refused(fn, args, op):
+    """Overwritten, it would keep the gradient of the values that are gone; under no_grad it is written, as torch's own calls do."""
+    from rnnt_amd import _torch_binding
+
+    _torch_binding.load()
+    leaf = args[-1].requires_grad_(True)
+    for out in (leaf, leaf * 1):
+        with pytest.raises(RuntimeError, match=op + " is for decoding and has no backward"):
+            fn(*args[:-1], out)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+            fn(*args[:-1], out)
+    with fwAD.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+        fn(*args[:-1], fwAD.make_dual(leaf.detach(), torch.ones_like(leaf)))
