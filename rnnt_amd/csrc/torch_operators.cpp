@@ -601,8 +601,7 @@ RulesIn rules_check(const Tensor &x, const MaybeTensor &bias_in, const MaybeTens
     TORCH_CHECK_VALUE((float)repetition > 0.f && std::isfinite((float)repetition), "repetition_penalty must be positive and finite");
     TORCH_CHECK_VALUE(std::isfinite((float)presence) && std::isfinite((float)frequency),
                       "presence_penalty and frequency_penalty must be finite");
-    if (values) check_tangents({&x, &in.bias}, op);  // (a token alone has no derivative)
-    check_no_grad({&written}, op);
+    if (values) check_no_grad({&x, &in.bias, &written}, op);  // (a token alone has no derivative)
     check_on_device(x, op);
     check_same_device(in.bias, x, "bias");
     check_same_device(in.allowed, x, "allowed");
@@ -650,7 +649,6 @@ Tensor process_logits_op(const Tensor &x, const MaybeTensor &bias, const MaybeTe
                          const MaybeTensor &out_in) {
     const RulesIn in = rules_check(x, bias, allowed, history, history_lens, repetition, presence, frequency, "process_logits", true,
                                    given(out_in));
-    check_no_grad({&x, &in.bias}, "process_logits");
     const c10::hip::HIPGuardMasqueradingAsCUDA guard(x.device());
     Tensor out;
     if (out_in.has_value()) {

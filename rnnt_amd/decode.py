@@ -45,7 +45,8 @@ def row_argmax(x: torch.Tensor, rules: Optional[LogitRules] = None) -> torch.Ten
 def row_max_logp(x: torch.Tensor, rules: Optional[LogitRules] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(int32[R], float32[R])``: argmax of every row of ``x[R, V]`` as :func:`row_argmax` gives it, and
     ``max(log_softmax(row))``, i.e. ``torch.max(F.log_softmax(x, -1), dim=1)`` in one launch; both of the logits as
-    ``rules`` change them if given."""
+    ``rules`` change them if given.  The score has no backward: without rules it carries no graph, with them logits (or a bias)
+    that require grad are refused in grad mode."""
     if rules is not None:
         return _torch_binding.load().row_rules(x, *_check(rules)._args(), True)
     if x.dim() != 2 or x.shape[0] < 1 or x.shape[1] < 1:

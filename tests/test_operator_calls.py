@@ -109,3 +109,15 @@ def test_a_buffer_that_autograd_follows_is_refused(fn, args, op):
             fn(*args[:-1], out)
     with fwAD.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
         fn(*args[:-1], fwAD.make_dual(leaf.detach(), torch.ones_like(leaf)))
+
+
+@pytest.mark.parametrize("op", ["row_max_logp", "process_logits", "row_argmax"])
+@pytest.mark.parametrize("name", ["x", "bias"])
+def test_values_without_a_backward_are_refused_where_a_gradient_is_asked_for(op, name):
+    """One answer from both calls that give values; a token has no derivative."""
+    call, tensors = calls()[op]
+    args = {**tensors, name: tensors[name].requires_grad_(True)}
+    with pytest.raises(RuntimeError, match="no CPU path" if op == "row_argmax" else op + " is for decoding and has no backward"):
+        call(**args)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
+        call(**args)
