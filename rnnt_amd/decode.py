@@ -92,7 +92,8 @@ def greedy_search_batch(encoder_output: torch.Tensor, decoder: Callable, joint: 
             ``decoder(tokens[n,1], hidden=hidden)`` -> ``(out[n,1,Hd], hidden)``, hidden a tensor or an
             ``(h, c)`` tuple shaped ``[layers, n, Hd]`` (or ``[layers, n, ...]``: :class:`rnnt_amd.PredictionNet`).
         rules: penalties, biases and masks on the logits (:class:`rnnt_amd.LogitRules`); an utterance's history is what it
-            has emitted, after ``rules.history`` if given.  A mask has to allow ``blank`` wherever no emission is due.
+            has emitted, after ``rules.history`` if given (which, with one token per frame, may be 65535 tokens long; without it the
+            limit is on what is emitted, and there is none where the penalties are neutral).  A mask has to allow ``blank`` wherever no emission is due.
     Returns:
         ``(predictions, mean(exp(score)), None, None)`` as the reference's 4-tuple (``:122-127``): token lists
         per utterance, and the batch mean of ``exp`` of each utterance's summed log-probabilities of its

@@ -16,6 +16,8 @@ import torch
 
 from . import _torch_binding
 
+_MAX_HISTORY = 65535   # the kernels' counters have 16 bits
+
 
 def pack_allowed(mask: torch.Tensor) -> torch.Tensor:
     """Bool ``[..., V]`` -> int32 ``[..., (V + 31) // 32]``: token ``v`` in bit ``v % 32`` of word ``v // 32``."""
@@ -75,10 +77,11 @@ def process_logits(x: torch.Tensor, rules: LogitRules, out: Optional[torch.Tenso
 
 
 class HistoryRules:
-    """``rules`` as a greedy search uses them: the history of every utterance grows with what it emits."""
+    """``rules`` as a greedy search uses them: the history of every utterance grows with what it emits.  It is kept, counted and
+    limited to 65535 tokens only where a penalty may look at it: neutral penalties change no logit, whatever was emitted."""
 
     def __init__(self, rules: LogitRules, batch: int, vocab: int, most: int, device):
-        self.rules = _check(rules)
+        self.rules, self.device = _check(rules), device
         self.tokens: List[List[int]] = [[] for _ in range(batch)]
         words = (vocab + 31) // 32
 
@@ -105,15 +108,19 @@ class HistoryRules:
         for name in ("history", "history_lens"):
             if getattr(rules, name) is not None and getattr(rules, name).dtype is not torch.int32:
                 raise TypeError(f"rules.{name} must be torch.int32")
-        if before + most > 65535:
+        if rules.history is not None and before + most > _MAX_HISTORY:
             raise ValueError("the history (with one token per frame) is longer than 65535 tokens")
-        self.history = torch.full((batch, before + most), -1, dtype=torch.int32, device=device)   # -1: no token
+        self.before = before
+        self.history = None
+        if rules.history is None and (rules.repetition_penalty, rules.presence_penalty, rules.frequency_penalty) == (1, 0, 0):
+            return
+        # -1: no token.  (room for as many emissions as can be counted: `most` frames may be more, and emit far less)
+        self.history = torch.full((batch, min(before + most, _MAX_HISTORY)), -1, dtype=torch.int32, device=device)
         if before:
             self.history[:, :before] = rules.history
             if rules.history_lens is not None:
                 late = torch.arange(before, device=device) >= rules.history_lens.to(device)[:, None]
                 self.history[:, :before].masked_fill_(late, -1)
-        self.before = before
 
     def _ask(self, b: int) -> None:
         words = self.grammar(list(self.tokens[b]))
@@ -122,10 +129,13 @@ class HistoryRules:
         self.allowed[b] = words.to(self.allowed.device)
 
     def emit(self, utterances: List[int], tokens: List[int]) -> None:
-        where = [self.before + len(self.tokens[b]) for b in utterances]
-        device = self.history.device
-        self.history[torch.tensor(utterances, device=device), torch.tensor(where, device=device)] = torch.tensor(
-            tokens, dtype=torch.int32, device=device)
+        if self.history is not None:
+            where = [self.before + len(self.tokens[b]) for b in utterances]
+            if max(where) >= _MAX_HISTORY:
+                raise ValueError("the history is longer than 65535 tokens: its counts have 16 bits")
+            device = self.history.device
+            self.history[torch.tensor(utterances, device=device), torch.tensor(where, device=device)] = torch.tensor(
+                tokens, dtype=torch.int32, device=device)
         for b, t in zip(utterances, tokens):
             self.tokens[b].append(t)
             if self.grammar is not None:
@@ -136,10 +146,11 @@ class HistoryRules:
         r = self.rules
         longest = self.before + max(len(self.tokens[b]) for b in utterances)
         every = len(utterances) == len(self.tokens)
-        sel = None if every else torch.tensor(utterances, device=self.history.device)
+        sel = None if every else torch.tensor(utterances, device=self.device)
 
         def pick(t):
             return t if t is None or t.dim() == 1 or every else t.index_select(0, sel)
 
-        return LogitRules(pick(self.bias), pick(self.allowed), pick(self.history)[:, :longest], None, r.repetition_penalty,
+        return LogitRules(pick(self.bias), pick(self.allowed), None if self.history is None else pick(self.history)[:, :longest],
+                          None, r.repetition_penalty,
                           r.presence_penalty, r.frequency_penalty)

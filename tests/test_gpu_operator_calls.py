@@ -1,5 +1,6 @@
 """GPU tests of how the prediction network's and the decoder's operators may be called: captured calls on leaves that the call
-has to lay out, forward-mode derivatives, results that a compiled graph uses only through the caller's buffer."""
+has to lay out, forward-mode derivatives, results that a compiled graph uses only through the caller's buffer, searches of
+more frames than a history has tokens."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -77,3 +78,46 @@ def test_a_compiled_graph_writes_the_callers_buffer(fn, args, op):
         for _ in range(3):      # (the first runs of a compiled graph record it, the later ones are optimised)
             graph(*args[:-1], out)
         assert torch.equal(out, want)
+
+
+def search_model(B, T, V=7, He=8, Hd=8):
+    import rnnt_amd
+
+    torch.manual_seed(11)
+    net = rnnt_amd.PredictionNet(V, 8, Hd, layers=1).to(DEV).eval()
+    joint = rnnt_amd.JointNet(He, 12, V, "sum").to(DEV).eval()
+    return net, joint, torch.randn(B, T, He, generator=torch.Generator().manual_seed(12)).to(DEV)
+
+
+def test_searches_of_more_frames_than_a_history_has_tokens():
+    """Rules that look at no history do not limit the frames; penalties limit the emissions."""
+    import rnnt_amd
+
+    T, V = 65700, 7
+    net, joint, enc = search_model(1, T)
+    quiet = torch.zeros(V, device=DEV)
+    quiet[0] = 100.0                                                 # blank at every frame
+    mask = rnnt_amd.pack_allowed(torch.ones(V, dtype=torch.bool)).to(DEV)
+    for rules in (rnnt_amd.LogitRules(bias=quiet), rnnt_amd.LogitRules(bias=quiet, allowed=mask),
+                  rnnt_amd.LogitRules(bias=quiet, allowed=lambda tokens: mask), rnnt_amd.LogitRules(bias=quiet, presence_penalty=1.0)):
+        assert rnnt_amd.greedy_decode(enc[0], T, net, joint, window=8192, rules=rules) == []
+    assert rnnt_amd.greedy_search_batch(enc, net, joint, window=8192, rules=rnnt_amd.LogitRules(bias=quiet))[0] == [[]]
+
+
+def test_neutral_penalties_give_what_a_counted_history_gives():
+    """With a history given, tokens are counted; neutral penalties then leave every logit as it is, to the bit."""
+    import rnnt_amd
+
+    net, joint, enc = search_model(3, 60)
+    bias = torch.randn(3, 7, generator=torch.Generator().manual_seed(13)).to(DEV)
+    allowed = lambda tokens: rnnt_amd.pack_allowed(torch.arange(7) != (tokens[-1] if tokens else 3))  # noqa: E731
+    history = torch.full((3, 1), 2, dtype=torch.int32, device=DEV)
+    for rules in (dict(bias=bias), dict(allowed=allowed), dict(bias=bias[0], allowed=allowed), {}):
+        free = rnnt_amd.greedy_search_batch(enc, net, joint, window=5, rules=rnnt_amd.LogitRules(**rules))
+        counted = rnnt_amd.greedy_search_batch(enc, net, joint, window=5, rules=rnnt_amd.LogitRules(**rules, history=history))
+        assert free[0] == counted[0] and torch.equal(free[1], counted[1])
+        assert sum(map(len, free[0])) > 3
+        one = {**rules, **({"bias": bias[:1]} if rules.get("bias") is bias else {})}
+        free, counted = (rnnt_amd.greedy_decode(enc[0], 60, net, joint, window=5, rules=rnnt_amd.LogitRules(**one, **h))
+                         for h in ({}, dict(history=history[:1])))
+        assert free == counted and free

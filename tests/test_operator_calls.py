@@ -121,3 +121,29 @@ def test_values_without_a_backward_are_refused_where_a_gradient_is_asked_for(op,
         call(**args)
     with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU path"):
         call(**args)
+
+
+def test_search_rules_keep_a_history_only_where_a_penalty_looks_at_it():
+    from rnnt_amd.rules import HistoryRules
+
+    frames = 70000                                                   # more than 16 bits count
+    words = torch.tensor([7], dtype=torch.int32)
+    said = []
+    kept = HistoryRules(R(bias=torch.ones(2, 9), allowed=lambda tokens: said.append(tokens) or words), 2, 9, frames, "cpu")
+    kept.emit([1], [4])
+    assert said == [[], [], [4]]                                     # a callable mask still follows what is emitted
+    now = kept.of([1])
+    assert now.history is None and now.bias.tolist() == [[1.0] * 9] and now.allowed.tolist() == [[7]]
+    kept.tokens[0] = [1] * 65535
+    kept.emit([0], [1])                                              # nothing is counted: no limit
+    for penalty in (dict(repetition_penalty=2.0), dict(presence_penalty=-1.0), dict(frequency_penalty=0.5)):
+        kept = HistoryRules(R(**penalty), 2, 9, frames, "cpu")
+        kept.emit([0, 1], [4, 5])
+        kept.emit([1], [6])
+        assert kept.of([0, 1]).history.tolist() == [[4, -1], [5, 6]]
+        kept.tokens[0] = [1] * 65534
+        kept.emit([0], [3])                                          # the last one that can be counted
+        assert kept.of([0]).history.shape == (1, 65535) and int(kept.of([0]).history[0, -1]) == 3
+        with pytest.raises(ValueError, match="longer than 65535"):
+            kept.emit([0], [3])
+    assert HistoryRules(R(presence_penalty=1.0), 2, 9, 5, "cpu").history.shape == (2, 5)
