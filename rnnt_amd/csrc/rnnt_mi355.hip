@@ -947,7 +947,7 @@ __device__ __forceinline__ u32x4 grad_chunk(const u32x4 &raw, const NodeCoef &n,
     constexpr int EPC = DT::EPC;
     float x[EPC];
     DT::unpack(raw, x);
-    // two logits per VALU instruction (v_pk_add_f32 / v_pk_fma_f32 / v_pk_mul_f32); only exp2 is scalar
+    // (in pairs; the build has no packed fp32 instructions, so a pair is two of each)
     const f32x2 m2 = {n.m, n.m}, k2 = {kLog2e, kLog2e}, n2 = {nl2, nl2}, sa2 = {n.sa, n.sa};
 #pragma unroll
     for (int j = 0; j < EPC; j += 2) {
