@@ -97,3 +97,18 @@ def test_no_packed_arithmetic(src, tmp_path, with_shipped_flags):
     assert kernels
     for name, body in kernels.items():
         assert not re.findall(r"^\s*v_pk_(?:add|mul|fma)_f32", body, re.M)[:5], name
+
+
+@pytest.mark.parametrize("src", SOURCES + operator_guards.SOURCES)
+def test_which_kernels_spill(src, compiled):
+    """Exactly: the scan's backward pass with 8 states (as its comment says) and, outside its vocabulary walk, the fused forward kernel
+    of the widest joint."""
+    result, _ = compiled(os.path.join(CSRC, src))
+    assert result.returncode == 0, result.stderr[-2000:]
+    names = re.findall(r"Function Name: (\S+)", result.stderr)
+    spills = [int(x) for x in re.findall(r"VGPRs Spill: (\d+)", result.stderr)]
+    assert names and len(names) == len(spills)
+    known = {"scan_backward_kernel": ("ELi8EEE", 5), "rnnt_fused_proj_k1": ("ELi512EEE", 7)}
+    for name, spilled in zip(names, spills):
+        limit = next((most for kernel, (form, most) in known.items() if kernel in name and form in name), 0)
+        assert spilled <= limit, (name, spilled)
