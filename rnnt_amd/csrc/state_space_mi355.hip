@@ -1126,7 +1126,17 @@ inline bool scan_shape_ok(int batch, int length, int dim, int state) {
            (batch * chunks * kChunk + 1) * 2 * state + ((long long)dim * (state + 2) + 4 * kWave) * 16 < (1ll << 32);
 }
 
-// Segments: none while the (sequence, 64 channels) pairs alone fill the chip.
+// Segments: none while the (sequence, 64 channels) pairs, a wave each, fill the chip; otherwise so many that about 10240 waves walk.
+// Both sides of each choice, in us, the kernels of a forward call / of a training pass (1024 channels, 16 states, bf16, all steps live):
+//   one segment from 2048 waves on   128 x 500 steps: whole 431 / 1319, cut 498 / 1856; 64 x 500 (1024 waves): 323 / 783 and 258 / 824 (a
+//                                    training pass would already rather be whole: 1020 and 1253 with 96 x 500)
+//   one segment up to 64 steps       32 x 41: whole 30 / 61, cut 31 / 82; 64 x 64: 43 / 117 and 55 / 152; it costs single sequences
+//                                    (1 x 41: 29 / 50 and 23 / 43); 1 x 96, above it: whole 54 / 93, cut 23 / 44
+//   10240 waves                      16 x 1500: 198 / 645, with 5120 212 / 674, with 2560 258 / 745, with 20480 199 / 640
+//   at least 16 steps, or 32 where   1 x 500 (512 waves of 16): 27 / 57 and, with 32, 39 / 76; 4 x 1500 (6016): 72 / 209 and 72 / 210;
+//   16 would give over 2048 waves    1 x 4095 x 1536 channels fp32 (6144): 82 / 236 and 75 / 221; 64 steps are slower in all (60 / 115, 90 / 233, 90 / 236)
+//   segments joined from 4096 work-  16 x 1500 (8192): one each 656, two 645, four 642; 32 x 1500: 1222, 1232, 1248.  It bounds the partial sums
+//   groups of the backward on        of dA, dD and ddt_bias, which each of them leaves, not the time
 inline ScanGeom scan_geometry(int batch, int length, int dim) {
     ScanGeom g = {};
     g.groups = groups_of(dim);
