@@ -449,7 +449,8 @@ rnntStatus_t rnnt_token_embedding_backward(const void *tokens, int tokens_64, lo
  * backward: grad_x / grad_initial in x's type, grad_weight [dim, width] / grad_bias [dim] fp32; grad_final (gradient of
  * final_state, NULL: none), grad_initial and grad_bias may be NULL.
  * workspace: rnnt_causal_conv_workspace_size bytes, 16-byte aligned.
- * step: one row per sequence, x [batch, dim] (x_batch apart); state_out may be the buffer of state (in place).
+ * step: one row per sequence, x [batch, dim] (x_batch apart; length, x_time and lengths are ignored); reads initial_state and writes
+ * final_state (both required; the same buffer: in place).
  */
 typedef struct {
     int batch, length, dim, width, silu, dtype;

@@ -103,7 +103,7 @@ void check_capture(std::initializer_list<const Tensor *> inputs, const char *op)
         const auto stream = accumulator->stream();
         TORCH_CHECK(!stream || stream->id() != 0 || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None,
                     "rnnt_amd.", op, " cannot be captured while a graph of an eager call on the default stream holds the same leaf: "
-                    "drop that call's results, or make it on another stream");
+                    "drop that call's results, make it on another stream, or capture under torch.no_grad() where no backward pass is captured");
     }
 }
 

@@ -18,7 +18,8 @@ from . import _torch_binding
 
 def token_embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
                     padding_idx: Optional[int] = None) -> torch.Tensor:
-    """``scale * weight[tokens]``, ``[*tokens.shape, dim]`` in ``weight``'s type; differentiable in ``weight``.
+    """``scale * weight[tokens]``, ``[*tokens.shape, dim]`` in ``weight``'s type; differentiable in ``weight`` (once, and not in
+    forward mode).
 
     Args:
         tokens: int32 or int64, any shape.  A token outside ``[0, vocab)`` gives a row of NaN and no gradient.

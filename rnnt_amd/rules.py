@@ -72,13 +72,14 @@ def _check(rules) -> LogitRules:
 
 def process_logits(x: torch.Tensor, rules: LogitRules, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``x[R, V]`` under ``rules``, computed in fp32 and rounded once to ``x``'s type (fp32, bf16 or fp16).  ``out`` may be
-    ``x`` itself.  No backward."""
+    ``x`` itself.  No backward: what requires grad (``out`` too) is refused in grad mode."""
     return _torch_binding.load().process_logits(x, *_check(rules)._args(), out)
 
 
 class HistoryRules:
     """``rules`` as a greedy search uses them: the history of every utterance grows with what it emits.  It is kept, counted and
-    limited to 65535 tokens only where a penalty may look at it: neutral penalties change no logit, whatever was emitted."""
+    limited to 65535 tokens only where a penalty may look at it (neutral penalties change no logit, whatever was emitted) or a history
+    is given."""
 
     def __init__(self, rules: LogitRules, batch: int, vocab: int, most: int, device):
         self.rules, self.device = _check(rules), device

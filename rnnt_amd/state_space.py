@@ -31,7 +31,7 @@ def causal_conv(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     ``p[t] = bias + sum_k weight[:, k] * xe[t + k]`` over ``xe = [initial_state; x]``, ``y = p * sigmoid(p)`` (or ``p``).
     ``final_state`` is the last ``width - 1`` rows of ``xe`` up to the sequence's length: the ``initial_state`` of what
     follows, and the ``state`` of :func:`causal_conv_step`.  Differentiable in ``x``, ``weight``, ``bias`` and
-    ``initial_state``, from both results.
+    ``initial_state``, from both results (once, and not in forward mode).
 
     Args:
         x: ``[B, L, dim]`` fp32, bf16 or fp16; rows may lie apart (half of a projection's output), channels adjacent.
@@ -47,7 +47,8 @@ def causal_conv_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor,
                      activation: Optional[str] = "silu",
                      state_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """:func:`causal_conv` of one token per sequence: ``x [B, dim]``, ``state [B, width - 1, dim]`` -> ``(y [B, dim], new
-    state)``.  ``state`` stays as it is unless it is also passed as ``state_out``.  No backward."""
+    state)``.  ``state`` stays as it is unless it is also passed as ``state_out``.  No backward: what requires grad
+    (``state_out`` too) is refused in grad mode."""
     return _torch_binding.load().causal_conv_step(x, state, weight, bias, _silu(activation), state_out)
 
 
@@ -58,7 +59,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     """Selective state space scan: ``(y [B, L, dim], final_state [B, dim, state] fp32)``.
 
     ``delta = softplus(dt + dt_bias)``; ``h[t] = exp(delta A) h[t-1] + delta x[t] B[t]``; ``y[t] = (<C[t], h[t]> + D x[t])
-    * z[t] sigmoid(z[t])`` (without ``z``: no factor).  Differentiable in every floating argument, from both results; the
+    * z[t] sigmoid(z[t])`` (without ``z``: no factor).  Differentiable in every floating argument, from both results (once, and not in forward mode); the
     backward reads the state before every 16th step, kept in fp32 (``4 state / 16`` bytes per element of ``x``).
 
     Args:
@@ -79,5 +80,5 @@ def selective_scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: t
                         state_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """:func:`selective_scan` of one token per sequence: ``x``, ``dt``, ``z`` ``[B, dim]``, ``B``, ``C`` ``[B, state]``,
     ``state [B, dim, state]`` fp32 -> ``(y [B, dim], new state)``.  ``state`` stays as it is unless it is also passed as
-    ``state_out``.  No backward."""
+    ``state_out``.  No backward: what requires grad (``state_out`` too) is refused in grad mode."""
     return _torch_binding.load().selective_scan_step(x, dt, A, B, C, state, D, z, dt_bias, state_out)

@@ -46,6 +46,25 @@ def test_capture_is_refused_for_a_leaf_that_the_call_lays_out(op, name):
     del held
 
 
+def test_a_forward_pass_is_captured_without_gradients_beside_an_eager_graph():
+    """Under no_grad there is no backward pass in the capture, and nothing to refuse."""
+    import rnnt_amd
+
+    for op, args in (("selective_scan", scan_args()), ("causal_conv", conv_args())):
+        leaves = {k: v.requires_grad_(True) for k, v in args.items()}
+        held = getattr(rnnt_amd, op)(**leaves)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph), torch.no_grad():
+            out = getattr(rnnt_amd, op)(**leaves)
+        for seed in range(3):
+            with torch.no_grad():
+                args["x"].copy_(torch.randn(args["x"].shape, generator=torch.Generator().manual_seed(seed)))
+                graph.replay()
+                torch.cuda.synchronize()
+                assert all(torch.equal(p, q) for p, q in zip(out, getattr(rnnt_amd, op)(**leaves)))
+        del held
+
+
 def test_a_tangent_is_refused_on_the_device():
     import rnnt_amd
 
