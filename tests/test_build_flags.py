@@ -6,6 +6,7 @@ import re
 import shlex
 import shutil
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 
@@ -43,24 +44,23 @@ def test_the_operators_guards_compile_what_is_shipped(shipped):
 
 @pytest.fixture(scope="module")
 def compiled(shipped, tmp_path_factory):
-    """source -> (hipcc's result with its report of resources, device assembly), compiled once for all guards."""
-    done, where, run = {}, tmp_path_factory.mktemp("asm"), subprocess.run
+    """source -> (hipcc's result with its report of resources, device assembly), compiled once for all guards, several at a time."""
+    where, run = tmp_path_factory.mktemp("asm"), subprocess.run
 
-    def one(path):
-        if path not in done:
-            asm = where / (os.path.basename(path) + ".s")
-            done[path] = run(["/opt/rocm/bin/hipcc", *shipped, "-Rpass-analysis=kernel-resource-usage", "--offload-device-only", "-S",
-                              "-o", str(asm), path], capture_output=True, text=True, timeout=900), asm
-        return done[path]
+    def one(src):
+        path, asm = os.path.join(CSRC, src), where / (src + ".s")
+        return path, (run(["/opt/rocm/bin/hipcc", *shipped, "-Rpass-analysis=kernel-resource-usage", "--offload-device-only", "-S",
+                           "-o", str(asm), path], capture_output=True, text=True, timeout=900), asm)
 
-    return one
+    with ThreadPoolExecutor(4) as pool:
+        return dict(pool.map(one, SOURCES + operator_guards.SOURCES))
 
 
 @pytest.fixture()
 def with_shipped_flags(compiled, monkeypatch):
     """The guards' own hipcc commands give what the shipped flags give for their source."""
     def shipped_run(command, **kw):
-        result, asm = compiled(command[-1])
+        result, asm = compiled[command[-1]]
         if "-S" in command:
             shutil.copy(asm, command[command.index("-o") + 1])
         return result
@@ -103,7 +103,7 @@ def test_no_packed_arithmetic(src, tmp_path, with_shipped_flags):
 def test_which_kernels_spill(src, compiled):
     """Exactly: the scan's backward pass with 8 states (as its comment says) and, outside its vocabulary walk, the fused forward kernel
     of the widest joint."""
-    result, _ = compiled(os.path.join(CSRC, src))
+    result, _ = compiled[os.path.join(CSRC, src)]
     assert result.returncode == 0, result.stderr[-2000:]
     names = re.findall(r"Function Name: (\S+)", result.stderr)
     spills = [int(x) for x in re.findall(r"VGPRs Spill: (\d+)", result.stderr)]
