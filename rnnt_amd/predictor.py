@@ -90,6 +90,7 @@ class PredictionNet(nn.Module):
     def forward(self, inputs: torch.Tensor, length: Optional[torch.Tensor] = None,
                 hidden: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
         """``inputs [B, U]`` tokens, ``length`` int32 or int64 ``[B]`` (None: all) -> ``(outputs [B, U, output_size], hidden)``.
+        Rows from ``length`` on hold any token of the vocabulary (one outside it gives NaN, in the Linear layers' gradients too).
         ``hidden`` is ``(conv [layers, B, width - 1, inner], scan [layers, B, inner, state])``, None: zeros; it is not changed."""
         if inputs.dim() != 2:
             raise ValueError("inputs must be [B, U]")
